@@ -419,6 +419,67 @@ int tc_attn_prefill_i8(const float *q, const int8_t *k8, const int8_t *v8,
                        uint64_t totalRows, float invSqrt, tc_stream stream);
 
 /* ------------------------------------------------------------------------- */
+/* paged K/V cache                                                             */
+/* ------------------------------------------------------------------------- */
+
+/* No counterpart in the reference (it keeps one session in one run of rows).  Many
+ * sequences share pools of pages: k / v [numPages][pageRows][nKV][hd], fp16 or (kvI8
+ * != 0) int8 with scales ks / vs [numPages][pageRows][nKV] f32 -- the arithmetic of
+ * tc_kv_append with kvHalf and of tc_kv_quantize_i8.  Row r of sequence b is row
+ * r % pageRows of page pages[b * pagesPerSeq + r / pageRows]; entries that no row
+ * needs are not looked at.  lens[b] counts the rows of sequence b, those of its new tokens
+ * included.  The token arrays of a call hold the new tokens of all sequences one
+ * behind another: sequence b has tokens [starts[b], starts[b + 1]), ascending, at rows
+ * lens[b] - n .. lens[b] - 1; starts == NULL: tokens / batch each.  Token rows behind
+ * starts[batch] are neither read nor written.  pages, lens and starts are DEVICE
+ * arrays, read at kernel time, so captured calls follow them.
+ * head_dim 64 (fp16 only), 128 or 256; pageRows a multiple of 8; pools 16-byte
+ * aligned.  A row whose page the table or the pool does not have, a length past
+ * pagesPerSeq * pageRows and a position past the rotation tables set the row-bound bit
+ * of tc_device_status: such a row is not stored, reads back as zero, and what attention
+ * makes of its sequence has no meaning; nothing outside the buffers is touched. */
+typedef struct tc_paged_kv {
+    void *k, *v;
+    float *ks, *vs;         /* NULL without kvI8 */
+    const int32_t *pages;   /* device [batch][pagesPerSeq] */
+    const uint32_t *lens;   /* device [batch] */
+    const uint32_t *starts; /* device [batch + 1] or NULL */
+    uint32_t batch, pagesPerSeq, numPages, pageRows, nKV, hd;
+    uint32_t tokens;        /* rows of the call's token arrays */
+    int kvI8;
+} tc_paged_kv;
+
+/* The new tokens' rows into their pages: k / v f32 [tokens][nKV][hd].  With tables
+ * (cosT / sinT [tableRows][hd/2]) K is rotated by the table row of its position as by
+ * tc_kv_append_rope.  q (nullable) f32 [tokens][nHeads][hd] is rotated along (copied
+ * without tables) into qOut, f32 (q itself allowed) or fp16 (qHalf != 0, the type that
+ * tc_attn_paged takes with half != 0).  Every array 16-byte aligned. */
+int tc_paged_kv_write(const tc_paged_kv *c, const float *k, const float *v, float *q,
+                      void *qOut, int qHalf, uint32_t nHeads, const float *cosT,
+                      const float *sinT, uint32_t tableRows, tc_stream stream);
+
+/* The last n_b = starts[b + 1] - starts[b] rows of every sequence back into kOut / vOut
+ * [tokens][nKV][hd], f32 or fp16 (outHalf != 0); int8 rows as byte x scale. */
+int tc_paged_kv_read(const tc_paged_kv *c, void *kOut, void *vOut, int outHalf,
+                     tc_stream stream);
+
+/* Causal attention of the new tokens over their sequences' rows (already written): the
+ * token at row r sees rows [0, r]; one that sees none gives zeros.  q / out
+ * [tokens][nHeads][hd], both f32 (results to f32 accuracy whatever the store) or both
+ * fp16 (half != 0: fp16 products, f32 sums and softmax).  maxTokens: the most
+ * new tokens of a sequence as far as the caller knows (0: unknown); it chooses the
+ * form of the launch, not the result's meaning.  Steps of one token, drafts, chunks and whole
+ * prompts may share a call.  Rows [0, lens[b]) have to hold finite numbers; what
+ * lies behind them may be anything.
+ * workspace: tc_attn_paged_workspace_bytes, 16-byte aligned, zeroed once before
+ * first use (every call leaves its counters zero); calls that may overlap need one each.
+ * At most 128 q heads per kv head. */
+int tc_attn_paged_workspace_bytes(size_t *bytes);
+int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half,
+                  uint32_t nHeads, uint32_t maxTokens, float invSqrt, void *workspace,
+                  size_t workspaceBytes, tc_stream stream);
+
+/* ------------------------------------------------------------------------- */
 /* the step in front of attention: Q/K RMSNorm + rotation, rotation tables      */
 /* ------------------------------------------------------------------------- */
 

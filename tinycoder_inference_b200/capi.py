@@ -154,6 +154,15 @@ class DecodeI8Batch(C.Structure):
     ]
 
 
+class PagedKv(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("ks", C.c_void_p), ("vs", C.c_void_p),
+        ("pages", C.c_void_p), ("lens", C.c_void_p), ("starts", C.c_void_p),
+        ("batch", C.c_uint32), ("pagesPerSeq", C.c_uint32), ("numPages", C.c_uint32), ("pageRows", C.c_uint32),
+        ("nKV", C.c_uint32), ("hd", C.c_uint32), ("tokens", C.c_uint32), ("kvI8", C.c_int),
+    ]
+
+
 # every symbol include/tc_attn.h declares, with its argument types
 _vp, _u32, _u64, _f, _i = C.c_void_p, C.c_uint32, C.c_uint64, C.c_float, C.c_int
 _sz_p = C.POINTER(C.c_size_t)
@@ -203,6 +212,10 @@ SIGNATURES = {
                                      _vp, _u64, _u64, _vp]),
     "tc_attn_prefill_kv": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _u64, _f, _i, _vp]),
     "tc_attn_prefill_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _u64, _f, _vp]),
+    "tc_paged_kv_write": (_i, [C.POINTER(PagedKv), _vp, _vp, _vp, _vp, _i, _u32, _vp, _vp, _u32, _vp]),
+    "tc_paged_kv_read": (_i, [C.POINTER(PagedKv), _vp, _vp, _i, _vp]),
+    "tc_attn_paged_workspace_bytes": (_i, [_sz_p]),
+    "tc_attn_paged": (_i, [C.POINTER(PagedKv), _vp, _vp, _i, _u32, _u32, _f, _vp, C.c_size_t, _vp]),
     "tc_attn_sigmoid_gate": (_i, [_vp, _vp, _u32, _u32, _u32, _vp]),
     "tc_context_request_init": (None, [C.POINTER(ContextRequest)]),
     "tc_kv_bytes_per_token": (_u64, [C.POINTER(ContextRequest), _u32, _u32]),

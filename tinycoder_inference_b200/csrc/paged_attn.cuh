@@ -1,0 +1,185 @@
+// paged_attn.cuh -- attention over a paged cache: the call as its kernels see it and how it is cut into work.
+//
+// An item is up to MR consecutive query rows of one kv head of one sequence; query row r of a sequence's kv head is q head
+// r % group of its token r / group, so the heads that share K and V sit side by side and one pass over the rows serves them.  A
+// unit is one tile of kPaTile cache rows of an item.  The units of all items in a row -- sequence, kv head, rows -- are cut into
+// equal runs, one per block: ragged lengths, single tokens and prompts fill the SMs alike.  An item that lies in several runs
+// is put together by the block of it that finishes last, from partials in the workspace.
+#pragma once
+
+#include "paged.cuh"
+
+namespace tc {
+
+constexpr uint32_t kPaTile = 64;  // cache rows of a unit
+
+struct PagedAttnParams {
+    PagedView c;
+    const void *q;   // [tokens][nHeads][hd] f32 / fp16
+    void *out;
+    const float *ks, *vs;
+    float *parts;            // two slots per block
+    unsigned int *tickets;   // one per block, zero between launches
+    uint32_t nHeads, group, box;  // box: cache rows of one TMA copy
+    uint32_t minRows, maxRows;    // the kernel takes the sequences with so many query rows per kv head (minRows .. maxRows)
+    float scaleLog2;
+    int half;                // q and out are fp16
+};
+
+#ifdef __CUDACC__
+// sum of (a i + b) / m over i = 0 .. n - 1, rounded down each
+__device__ __forceinline__ uint64_t floorSum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    uint64_t sum = 0;
+    for (;;) {
+        if (a >= m) sum += n * (n - 1) / 2 * (a / m), a %= m;
+        if (b >= m) sum += n * (b / m), b %= m;
+        const uint64_t top = a * n + b;
+        if (top < m) return sum;
+        n = top / m, b = top % m;
+        const uint64_t x = m;
+        m = a, a = x;
+    }
+}
+
+// The work of one sequence: query rows per kv head, rows cached, and what its items need.
+struct PagedSeq {
+    uint32_t rows, len;  // query rows of a kv head (new tokens x group); cache rows
+    int32_t before;      // cache rows ahead of the new tokens; negative: the first tokens see nothing
+    uint32_t token0;     // first token
+
+    // cache rows that the last of query rows [.., end) sees
+    __device__ __forceinline__ uint32_t sees(uint32_t end, uint32_t group) const {
+        const int32_t n = before + static_cast<int32_t>((end - 1u) / group) + 1;
+        return n > 0 ? static_cast<uint32_t>(n) : 0u;
+    }
+    template <uint32_t MR>
+    __device__ __forceinline__ uint32_t items() const { return (rows + MR - 1u) / MR; }
+    // tiles of item m: one at least, which writes the zeros of rows that see nothing.  Where `before` is negative every item is
+    // counted with the tiles of the whole sequence, so that the sum below keeps its closed form.
+    template <uint32_t MR>
+    __device__ __forceinline__ uint32_t tiles(uint32_t m, uint32_t group) const {
+        const uint32_t n = before < 0 ? len : sees(min((m + 1u) * MR, rows), group);
+        return max(1u, (n + kPaTile - 1u) / kPaTile);
+    }
+    // tiles of items 0 .. m - 1
+    template <uint32_t MR>
+    __device__ __forceinline__ uint64_t tilesBefore(uint32_t m, uint32_t group) const {
+        if (m == 0u) return 0u;
+        if (before < 0) return static_cast<uint64_t>(m) * tiles<MR>(0, group);
+        const bool all = m == items<MR>();
+        const uint32_t n = all ? m - 1u : m;
+        uint64_t sum = all ? tiles<MR>(m - 1u, group) : 0u;
+        // item i sees before + ((i + 1) MR - 1) / group + 1 rows: floor((group (before + kPaTile) + (i + 1) MR - 1) / (kPaTile group)) tiles
+        if (n > 0u) sum += floorSum(n, static_cast<uint64_t>(kPaTile) * group, MR, static_cast<uint64_t>(group) * (static_cast<uint32_t>(before) + kPaTile) + MR - 1u);
+        return sum;
+    }
+    template <uint32_t MR>
+    __device__ __forceinline__ uint64_t tilesAll(uint32_t group) const { return rows == 0u ? 0u : tilesBefore<MR>(items<MR>(), group); }
+};
+
+__device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, uint32_t b) {
+    const uint32_t s0 = seqStart(p.c, b), s1 = min(seqStart(p.c, b + 1u), p.c.tokens);
+    PagedSeq s;
+    const uint32_t n = s1 > s0 ? s1 - s0 : 0u, most = p.c.pagesPerSeq * p.c.pageRows;
+    uint32_t len = __ldg(p.c.lens + b);
+    if (len > most) {  // more rows than the table has pages for
+        atomicOr(p.c.err, kDevErrRowBound);
+        len = most;
+    }
+    s.rows = n * p.group;
+    if (s.rows < p.minRows || s.rows > p.maxRows) s.rows = 0u;
+    s.len = len;
+    s.before = static_cast<int32_t>(len) - static_cast<int32_t>(n);
+    s.token0 = s0;
+    return s;
+}
+
+// A walk over a block's run of units, item by item; every warp makes its own, in step.  MR: query rows of an item.
+template <uint32_t MR>
+struct PagedWalk {
+    uint64_t total, at, end;  // units of the launch; the block's next and last
+    uint32_t blocks;          // blocks with work
+    uint32_t seq, kvHead, item;
+    uint64_t item0;           // first unit of the item
+    uint32_t tiles;           // its tiles
+    PagedSeq s;
+
+    __device__ __forceinline__ uint64_t firstOf(uint32_t block) const { return static_cast<uint64_t>(block) * total / blocks; }
+    __device__ __forceinline__ uint32_t blockOf(uint64_t unit) const { return static_cast<uint32_t>(((unit + 1u) * blocks - 1u) / total); }
+
+    // All lanes of the warp.  False: nothing to do.
+    __device__ __forceinline__ bool begin(const PagedAttnParams &p) {
+        const uint32_t lane = threadIdx.x & 31u;
+        uint64_t sum = 0;
+        for (uint32_t b0 = 0; b0 < p.c.batch; b0 += 32u)
+            if (b0 + lane < p.c.batch) sum += pagedSeq(p, b0 + lane).template tilesAll<MR>(p.group) * p.c.nKV;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        total = sum;
+        if (total == 0u) return false;
+        blocks = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x), total));
+        if (blockIdx.x >= blocks) return false;
+        at = firstOf(blockIdx.x), end = firstOf(blockIdx.x + 1u);
+        // the sequence that holds unit `at`
+        uint64_t base = 0;
+        for (uint32_t b0 = 0;; b0 += 32u) {
+            uint64_t mine = 0;
+            if (b0 + lane < p.c.batch) mine = pagedSeq(p, b0 + lane).template tilesAll<MR>(p.group) * p.c.nKV;
+            uint64_t upTo = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t x = __shfl_up_sync(0xffffffffu, upTo, o);
+                if (lane >= static_cast<uint32_t>(o)) upTo += x;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, base + upTo > at);
+            if (past != 0u) {
+                const int l = __ffs(past) - 1;
+                seq = b0 + l;
+                base += __shfl_sync(0xffffffffu, upTo - mine, l);
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, upTo, 31);
+            if (b0 + 32u >= p.c.batch) return false;  // (not reached: `at` lies below the sum)
+        }
+        s = pagedSeq(p, seq);
+        const uint64_t per = s.template tilesAll<MR>(p.group);
+        kvHead = static_cast<uint32_t>((at - base) / per);
+        const uint64_t in = at - base - kvHead * per;
+        uint32_t lo = 0, hi = s.template items<MR>() - 1u;  // the last item whose first tile is not behind `in`
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi + 1u) / 2u;
+            if (s.template tilesBefore<MR>(mid, p.group) <= in) lo = mid;
+            else hi = mid - 1u;
+        }
+        item = lo;
+        item0 = base + kvHead * per + s.template tilesBefore<MR>(item, p.group);
+        tiles = s.template tiles<MR>(item, p.group);
+        return true;
+    }
+    // Tiles [first, last) of the item are the block's.
+    __device__ __forceinline__ uint32_t first() const { return static_cast<uint32_t>(at - item0); }
+    __device__ __forceinline__ uint32_t last() const { return static_cast<uint32_t>(min(end - item0, static_cast<uint64_t>(tiles))); }
+    // On to the next item; false: the run is done.
+    __device__ __forceinline__ bool next(const PagedAttnParams &p) {
+        item0 += tiles;
+        at = item0;
+        if (at >= end) return false;
+        if (++item == s.template items<MR>()) {
+            item = 0;
+            if (++kvHead == p.c.nKV) {
+                kvHead = 0;
+                do {
+                    if (++seq >= p.c.batch) return false;  // (not reached: the run is not done)
+                    s = pagedSeq(p, seq);
+                } while (s.rows == 0u);
+            }
+        }
+        tiles = s.template tiles<MR>(item, p.group);
+        return true;
+    }
+};
+#endif
+
+int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v);  // maps of the pools, `box` rows a copy
+
+}  // namespace tc

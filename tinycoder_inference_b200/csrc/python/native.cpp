@@ -15,7 +15,9 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <type_traits>
 #include <utility>
 
@@ -188,12 +190,181 @@ PyObject *decodeI8Batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// The paged cache of a call, from its tensors: pools [pages][rows][kv heads][head_dim], tables int32 [batch][pages per sequence], and
+// `like`, whose first dimension is the call's tokens.  What a layout or a type would make wrong is refused here; sizes are the library's to check.
+bool pagedTensor(PyObject *o, const char *name, at::ScalarType type, int64_t dims, const at::Tensor **out, const at::Device *dev = nullptr) {
+    if (!THPVariable_Check(o)) {
+        PyErr_Format(PyExc_TypeError, "%s: tensor expected, got %s", name, Py_TYPE(o)->tp_name);
+        return false;
+    }
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || !t.is_contiguous()) {
+        PyErr_Format(PyExc_AssertionError, "%s: device-resident contiguous tensor required", name);
+        return false;
+    }
+    if (t.scalar_type() != type || t.dim() != dims) {
+        PyErr_Format(PyExc_ValueError, "%s: %s of %lld dimensions expected", name, c10::toString(type), static_cast<long long>(dims));
+        return false;
+    }
+    if (dev != nullptr && t.device() != *dev) {
+        PyErr_Format(PyExc_ValueError, "%s: not on the device of the cache", name);
+        return false;
+    }
+    *out = &t;
+    return true;
+}
+struct Paged {
+    tc_paged_kv c;
+    at::Device dev = at::Device(at::kCUDA);
+    bool fail(const char *text) {
+        PyErr_SetString(PyExc_ValueError, text);
+        return false;
+    }
+    bool same(const at::Tensor &t, std::initializer_list<int64_t> sizes, const char *name) {
+        if (t.sizes() != at::IntArrayRef(sizes.begin(), sizes.size())) {
+            PyErr_Format(PyExc_ValueError, "%s: another shape expected", name);
+            return false;
+        }
+        return true;
+    }
+    // kc, vc, ks, vs, pages, lens, starts
+    bool take(PyObject *const *a) {
+        memset(&c, 0, sizeof(c));
+        const at::Tensor *kc, *vc, *pages, *lens, *t;
+        if (!THPVariable_Check(a[0])) return fail("the cache is a tensor");
+        const auto type = THPVariable_Unpack(a[0]).scalar_type();
+        if (type != at::kHalf && type != at::kChar) return fail("the cache is fp16 or int8");
+        if (!pagedTensor(a[0], "k cache", type, 4, &kc)) return false;
+        dev = kc->device();
+        if (dev.index() != c10::cuda::current_device()) return fail("the cache is not on the current device");
+        if (!pagedTensor(a[1], "v cache", type, 4, &vc, &dev) || !pagedTensor(a[4], "pages", at::kInt, 2, &pages, &dev) ||
+            !pagedTensor(a[5], "lens", at::kInt, 1, &lens, &dev))
+            return false;
+        if (vc->sizes() != kc->sizes()) return fail("k and v caches of different shapes");
+        if (lens->size(0) != pages->size(0)) return fail("lens and pages of different batches");
+        for (const auto *x : {kc, pages})
+            for (const int64_t n : x->sizes())
+                if (n > 0x7fffffffll) return fail("a dimension of the cache is too long");
+        c.kvI8 = type == at::kChar;
+        if (c.kvI8) {
+            for (int i = 2; i < 4; ++i) {
+                if (!pagedTensor(a[i], i == 2 ? "ks" : "vs", at::kFloat, 3, &t, &dev) || !same(*t, {kc->size(0), kc->size(1), kc->size(2)}, "scales")) return false;
+                (i == 2 ? c.ks : c.vs) = static_cast<float *>(t->data_ptr());
+            }
+        } else if (a[2] != Py_None || a[3] != Py_None) {
+            return fail("scales belong to an int8 cache");
+        }
+        if (a[6] != Py_None) {
+            if (!pagedTensor(a[6], "starts", at::kInt, 1, &t, &dev) || !same(*t, {lens->size(0) + 1}, "starts")) return false;
+            c.starts = static_cast<const uint32_t *>(t->data_ptr());
+        }
+        c.k = kc->data_ptr(), c.v = vc->data_ptr();
+        c.pages = static_cast<const int32_t *>(pages->data_ptr());
+        c.lens = static_cast<const uint32_t *>(lens->data_ptr());
+        c.numPages = static_cast<uint32_t>(kc->size(0)), c.pageRows = static_cast<uint32_t>(kc->size(1));
+        c.nKV = static_cast<uint32_t>(kc->size(2)), c.hd = static_cast<uint32_t>(kc->size(3));
+        c.batch = static_cast<uint32_t>(pages->size(0)), c.pagesPerSeq = static_cast<uint32_t>(pages->size(1));
+        return true;
+    }
+    // a token array [tokens][heads (0: any)][hd]; the first one says how many tokens there are
+    bool rows(PyObject *o, const char *name, at::ScalarType type, int64_t heads, bool first, const at::Tensor **out) {
+        if (!pagedTensor(o, name, type, 3, out, &dev)) return false;
+        const at::Tensor &t = **out;
+        if (t.size(0) > 0x7fffffffll || t.size(1) > 0x7fffffffll) return fail("too many tokens or heads");
+        if (first) c.tokens = static_cast<uint32_t>(t.size(0));
+        return same(t, {first ? t.size(0) : static_cast<int64_t>(c.tokens), heads ? heads : t.size(1), static_cast<int64_t>(c.hd)}, name);
+    }
+    static bool halfOrFloat(PyObject *o, at::ScalarType *type) {
+        *type = THPVariable_Check(o) ? THPVariable_Unpack(o).scalar_type() : at::kFloat;
+        if (*type == at::kHalf || *type == at::kFloat) return true;
+        PyErr_SetString(PyExc_ValueError, "f32 or fp16 expected");
+        return false;
+    }
+};
+
+// paged_write(kc, vc, ks, vs, pages, lens, starts, k, v, q, q_out, cosT, sinT)
+PyObject *pagedWrite(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 13) {
+        PyErr_SetString(PyExc_TypeError, "paged_write: 13 arguments expected");
+        return nullptr;
+    }
+    Paged p;
+    const at::Tensor *k, *v, *q = nullptr, *qOut = nullptr, *cosT = nullptr, *sinT = nullptr;
+    at::ScalarType outType = at::kFloat;
+    if (!p.take(a) || !p.rows(a[7], "k", at::kFloat, p.c.nKV, true, &k) || !p.rows(a[8], "v", at::kFloat, p.c.nKV, false, &v)) return nullptr;
+    if (a[9] != Py_None &&
+        (!p.rows(a[9], "q", at::kFloat, 0, false, &q) || !Paged::halfOrFloat(a[10], &outType) || !p.rows(a[10], "q_out", outType, q->size(1), false, &qOut)))
+        return nullptr;
+    if ((a[11] == Py_None) != (a[12] == Py_None)) return p.fail("cosT and sinT come together"), nullptr;
+    if (a[11] != Py_None) {
+        if (!pagedTensor(a[11], "cosT", at::kFloat, 2, &cosT, &p.dev) || !pagedTensor(a[12], "sinT", at::kFloat, 2, &sinT, &p.dev) ||
+            !p.same(*cosT, {cosT->size(0), static_cast<int64_t>(p.c.hd / 2)}, "cosT") || !p.same(*sinT, {cosT->size(0), cosT->size(1)}, "sinT"))
+            return nullptr;
+        if (cosT->size(0) > 0x7fffffffll) return p.fail("too many table rows"), nullptr;
+    }
+    auto f = [](const at::Tensor *t) { return t != nullptr ? static_cast<float *>(t->data_ptr()) : nullptr; };
+    const tc_stream st = currentStream();
+    return PyLong_FromLong(unlocked([&] {
+        return tc_paged_kv_write(&p.c, f(k), f(v), f(q), qOut != nullptr ? qOut->data_ptr() : nullptr, outType == at::kHalf,
+                                 q != nullptr ? static_cast<uint32_t>(q->size(1)) : 0u, f(cosT), f(sinT),
+                                 cosT != nullptr ? static_cast<uint32_t>(cosT->size(0)) : 0u, st);
+    }));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_read(kc, vc, ks, vs, pages, lens, starts, k_out, v_out)
+PyObject *pagedRead(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9) {
+        PyErr_SetString(PyExc_TypeError, "paged_read: 9 arguments expected");
+        return nullptr;
+    }
+    Paged p;
+    const at::Tensor *k, *v;
+    at::ScalarType type;
+    if (!p.take(a) || !Paged::halfOrFloat(a[7], &type) || !p.rows(a[7], "k_out", type, p.c.nKV, true, &k) ||
+        !p.rows(a[8], "v_out", type, p.c.nKV, false, &v))
+        return nullptr;
+    const tc_stream st = currentStream();
+    return PyLong_FromLong(unlocked([&] { return tc_paged_kv_read(&p.c, k->data_ptr(), v->data_ptr(), type == at::kHalf, st); }));
+    END_HANDLE_TH_ERRORS
+}
+
+// attn_paged(kc, vc, ks, vs, pages, lens, starts, q, out, workspace, max_tokens, invSqrt)
+PyObject *attnPaged(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 12) {
+        PyErr_SetString(PyExc_TypeError, "attn_paged: 12 arguments expected");
+        return nullptr;
+    }
+    Paged p;
+    const at::Tensor *q, *out, *ws;
+    at::ScalarType type;
+    uint32_t maxTokens;
+    float invSqrt;
+    if (!p.take(a) || !Paged::halfOrFloat(a[7], &type) || !p.rows(a[7], "q", type, 0, true, &q) || !p.rows(a[8], "out", type, q->size(1), false, &out) ||
+        !pagedTensor(a[9], "workspace", at::kFloat, 1, &ws, &p.dev) || !toArg(a[10], &maxTokens))
+        return nullptr;
+    if (a[11] == Py_None) invSqrt = 1.0f / std::sqrt(static_cast<float>(p.c.hd));
+    else if (!toArg(a[11], &invSqrt)) return nullptr;
+    const tc_stream st = currentStream();
+    return PyLong_FromLong(unlocked([&] {
+        return tc_attn_paged(&p.c, q->data_ptr(), out->data_ptr(), type == at::kHalf, static_cast<uint32_t>(q->size(1)), maxTokens, invSqrt, ws->data_ptr(),
+                             static_cast<size_t>(ws->numel()) * 4, st);
+    }));
+    END_HANDLE_TH_ERRORS
+}
+
 #define TC_FAST(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 #define TC_WRAP(name, fn) TC_FAST(name, Wrap<fn>::py)
 PyMethodDef kMethods[] = {
         TC_FAST("attend", attend),
         TC_FAST("begin", begin),
         TC_FAST("decode_i8_batch", decodeI8Batch),
+        TC_FAST("paged_write", pagedWrite),
+        TC_FAST("paged_read", pagedRead),
+        TC_FAST("attn_paged", attnPaged),
         TC_WRAP("clear", tc_kv_session_clear),
         TC_WRAP("kv_append", tc_kv_append),
         TC_WRAP("kv_append_rope", tc_kv_append_rope),

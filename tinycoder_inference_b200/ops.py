@@ -266,6 +266,37 @@ def sigmoid_gate(attnOut, qGate, seqLen, nHeads, hd):
     check(_n.sigmoid_gate(attnOut, qGate, seqLen, nHeads, hd))
 
 
+# ---- paged K/V cache ------------------------------------------------------------
+#
+# Many sequences in shared pools of pages: kc, vc [pages][rows][nKV][hd] fp16, or int8 with scales ks, vs
+# [pages][rows][nKV] f32.  pages int32 [batch][pages per sequence], lens int32 [batch] (rows, new tokens included).
+# The token arrays hold the new tokens of all sequences one behind another, split by starts int32 [batch + 1]
+# (None: the same number each); they sit in the last rows of their sequences.
+
+def paged_write(k, v, kc, vc, pages, lens, starts=None, ks=None, vs=None, q=None, q_out=None, cosT=None, sinT=None):
+    """New tokens' k, v f32 [tokens][nKV][hd] into their pages, K rotated by its position's row of cosT / sinT
+    [rows][hd/2] if given.  q f32 [tokens][nHeads][hd] is rotated along into q_out (f32 or fp16; default: in place)."""
+    check(_n.paged_write(kc, vc, ks, vs, pages, lens, starts, k, v, q, q if q_out is None else q_out, cosT, sinT))
+
+
+def paged_read(kc, vc, pages, lens, k_out, v_out, starts=None, ks=None, vs=None):
+    """The last rows of every sequence (as many as starts says) into k_out, v_out [tokens][nKV][hd], f32 or fp16."""
+    check(_n.paged_read(kc, vc, ks, vs, pages, lens, starts, k_out, v_out))
+
+
+def paged_workspace(device=None):
+    """What attn_paged calls need, one for all calls that follow one another."""
+    n = C.c_size_t(0)
+    check(lib.tc_attn_paged_workspace_bytes(C.byref(n)))
+    return torch.zeros(n.value // 4, dtype=torch.float32, device=device or torch.device("cuda", torch.cuda.current_device()))
+
+
+def attn_paged(q, kc, vc, pages, lens, out, ws, starts=None, max_tokens=0, ks=None, vs=None, invSqrt=None):
+    """Causal attention of the new tokens over their sequences' rows.  q, out [tokens][nHeads][hd], both f32 or both
+    fp16.  max_tokens: the most new tokens of a sequence as far as the caller knows (0: unknown)."""
+    check(_n.attn_paged(kc, vc, ks, vs, pages, lens, starts, q, out, ws, max_tokens, invSqrt))
+
+
 # ---- planner (host) -------------------------------------------------------------
 
 def context_request(**kw) -> capi.ContextRequest:
