@@ -471,8 +471,8 @@ int tc_paged_kv_read(const tc_paged_kv *c, void *kOut, void *vOut, int outHalf,
  * form of the launch, not the result's meaning.  Steps of one token, drafts, chunks and whole
  * prompts may share a call.  Rows [0, lens[b]) have to hold finite numbers; what
  * lies behind them may be anything.
- * workspace: tc_attn_paged_workspace_bytes, 16-byte aligned, zeroed once before
- * first use (every call leaves its counters zero); calls that may overlap need one each.
+ * workspace: tc_attn_paged_workspace_bytes, 16-byte aligned, whatever it holds; calls that
+ * may overlap need one each.
  * At most 128 q heads per kv head. */
 int tc_attn_paged_workspace_bytes(size_t *bytes);
 int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half,

@@ -21,14 +21,15 @@
 #include <cstring>
 
 #include "paged_attn.cuh"
+#include "tc_tcgen05.cuh"
 
 namespace tc {
 
 constexpr int kPaThreads = 160;       // four consumer warps, one producer warp
-// The workspace: two partials per block of the widest grid, then a ticket per block.
+// The workspace: two partials per block of the widest grid, then what the merge finds per block.
 constexpr int kPagedSMs = 148;
 constexpr size_t kPagedParts = size_t(2) * kPagedSMs * 2 * 64 * (128 + 2);  // f32
-constexpr size_t kPagedWorkspace = kPagedParts * 4 + size_t(kPagedSMs) * 2 * 4;
+constexpr size_t kPagedWorkspace = kPagedParts * 4 + size_t(kPagedSMs) * 2 * sizeof(PagedJoin);
 constexpr float kPaOff = 13.0f;       // p is held as 2^13 p: its fp16 pair keeps 11 + 11 bits down to p = 2^-27
 
 template <int HD, bool I8, bool PAIR, int WM>
@@ -46,25 +47,10 @@ struct PaL {
     static constexpr int kBuf = kScales + (I8 ? NST * 512 : 0);    // [warp][16][36] f32
     static constexpr int kMl = kBuf + 4 * 16 * 36 * 4;             // [warp][16] (m, l)
     static constexpr int kBars = kMl + 4 * 16 * 8;
-    static constexpr int kFlag = kBars + 2 * NST * 8;
-    static constexpr int kTotal = kFlag + 16 + 1024;
+    static constexpr int kTotal = kBars + 2 * NST * 8 + 1024;
     static constexpr int kBlocks = HD == 256 ? 1 : 2;
     static_assert(kBlocks * (kTotal + 1024) <= 228 * 1024, "shared memory of an SM");
 };
-
-// Bounded wait, as in prefill_f16.cu: 2^18 polls of up to 20 us, given up as soon as another thread has.
-__device__ __forceinline__ bool paWait(uint64_t *bar, uint32_t parity, unsigned int *err, uint32_t bit) {
-    if (mbarTryWait(bar, parity)) return true;
-#pragma unroll 1
-    for (uint32_t i = 0; i < (1u << 18); ++i) {
-        if (mbarTryWait(bar, parity)) return true;
-        if ((i & 63u) == 63u &&
-            (*reinterpret_cast<volatile unsigned int *>(err) & (kDevErrFullWait | kDevErrEmptyWait | kDevErrMmaWait)) != 0u)
-            return false;
-    }
-    atomicOr(err, bit);
-    return false;
-}
 
 __device__ __forceinline__ uint4 ldShared4(uint32_t addr) {
     uint4 v;
@@ -80,62 +66,113 @@ __device__ __forceinline__ uint32_t sub1152(uint32_t x) {
 __device__ __forceinline__ uint32_t bytesLo(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4140)); }
 __device__ __forceinline__ uint32_t bytesHi(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4342)); }
 
-// Block-wide among the consumer warps: the last of an item's blocks puts its partials together.
-// Slot of a partial: acc [MR][HD], m [MR], l [MR], relative to m.
-template <int HD, int MR>
-__device__ __forceinline__ void pagedStore(const PagedAttnParams &p, const PagedSeq &s, uint32_t kvHead, uint32_t r, uint32_t dim, const float4 &x) {
-    const uint32_t tok = s.token0 + r / p.group, head = kvHead * p.group + r % p.group;
-    const size_t at = (static_cast<size_t>(tok) * p.nHeads + head) * HD + dim;
+__device__ __forceinline__ void pagedStore(const PagedAttnParams &p, uint32_t hd, uint32_t token0, uint32_t kvHead, uint32_t r, uint32_t dim, const float4 &x) {
+    const uint32_t tok = token0 + r / p.group, head = kvHead * p.group + r % p.group;
+    const size_t at = (static_cast<size_t>(tok) * p.nHeads + head) * hd + dim;
     if (p.half) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + at) = make_uint2(packHalf2(x.x, x.y), packHalf2(x.z, x.w));
     else *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = x;
 }
 
-template <int HD, int MR>
-__device__ __forceinline__ void pagedMerge(const PagedAttnParams &p, const PagedWalk<MR> &w, uint32_t c0, uint32_t count) {
-    constexpr size_t kSlot = static_cast<size_t>(MR) * (HD + 2);
+// The partials of the items that several blocks had a part in: block (i, y) takes item i's rows y, y + gridDim.y, ... (in steps of 8 / W).
+// W warps share a row, each a W-th of its partials: few rows of many parts (a step of one long session: 74) are as much a chain of loads
+// as many rows of two.
+template <int HD>
+__global__ void __launch_bounds__(256) pagedMergeKernel(const __grid_constant__ PagedAttnParams p) {
+    constexpr int V = HD / 128 ? HD / 128 : 1;  // float4 of a lane
+    __shared__ float4 sAcc[8][V * 32];
+    __shared__ float2 sMl[8];
+    gridDepWait();
+    gridDepLaunch();
+    const PagedJoin j = p.joins[blockIdx.x];
+    if (j.count == 0u) return;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    // block c0 ends with the item (its second slot), the others begin with it
-    auto part = [&](uint32_t c) { return p.parts + (2u * static_cast<size_t>(c0 + c) + (c == 0u ? 1u : 0u)) * kSlot; };
-    constexpr int V = HD / 128 ? HD / 128 : 1;                       // float4 of a lane
-    for (uint32_t i = warp; i < MR; i += 4u) {
-        const uint32_t r = w.item * MR + i;
-        if (r >= w.s.rows) break;
-        float M = -INFINITY;
-        for (uint32_t c = lane; c < count; c += 32u) M = fmaxf(M, __ldcg(part(c) + MR * HD + i));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float Mu = M == -INFINITY ? 0.0f : M;
+    const size_t slot = static_cast<size_t>(j.mr) * (HD + 2);
+    auto part = [&](uint32_t c) { return p.parts + (2u * static_cast<size_t>(blockIdx.x + c) + (c == 0u ? 1u : 0u)) * slot; };
+    const uint32_t W = j.count <= 8u ? 1u : j.count <= 16u ? 2u : j.count <= 32u ? 4u : 8u, perPass = 8u / W, mine = warp % W;
+    const uint32_t rows = min(j.mr, j.rows - j.row0);
+    for (uint32_t i0 = blockIdx.y * perPass; i0 < rows; i0 += gridDim.y * perPass) {
+        const uint32_t i = i0 + warp / W;
+        float M = -INFINITY, L = 0.0f;
         float4 acc[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-        float L = 0.0f;
-        for (uint32_t cb = 0; cb < count; cb += 32u) {
-            float wc = 0.0f;
-            if (cb + lane < count) {
-                wc = fastExp2(__ldcg(part(cb + lane) + MR * HD + i) - Mu);  // (-inf: 0)
-                L = fmaf(wc, __ldcg(part(cb + lane) + MR * HD + MR + i), L);
-            }
-            const uint32_t n = min(32u, count - cb);
-#pragma unroll 8
-            for (uint32_t c = 0; c < n; ++c) {
-                const float f = __shfl_sync(0xffffffffu, wc, c);
-                const float *a = part(cb + c) + i * HD;
+        if (i < rows) {
+            // 32 W partials at a time; the first accumulators are under way before the maxima that weigh them
+            constexpr uint32_t A = HD == 256 ? 4 : 8;
+            for (uint32_t cb = mine; cb < j.count; cb += 32u * W) {
+                const uint32_t n = min(32u, (j.count - cb + W - 1u) / W);
+                auto load = [&](uint32_t c, float4(&x)[V]) {
+                    const float4 *a = reinterpret_cast<const float4 *>(part(cb + W * c) + static_cast<size_t>(i) * HD);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (HD < 128 && lane >= HD / 4u) continue;
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(a) + v * 32 + lane);
-                    acc[v].x = fmaf(f, x.x, acc[v].x), acc[v].y = fmaf(f, x.y, acc[v].y);
-                    acc[v].z = fmaf(f, x.z, acc[v].z), acc[v].w = fmaf(f, x.w, acc[v].w);
+                    for (int v = 0; v < V; ++v) x[v] = HD >= 128 || lane < HD / 4u ? a[v * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+                };
+                float4 x[A][V];
+#pragma unroll
+                for (uint32_t u = 0; u < A; ++u)
+                    if (u < n) load(u, x[u]);
+                float m = -INFINITY, l = 0.0f;
+                if (lane < n) m = part(cb + W * lane)[j.mr * HD + i], l = part(cb + W * lane)[j.mr * HD + j.mr + i];
+                float top = fmaxf(m, M);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float Mu = top == -INFINITY ? 0.0f : top, keep = fastExp2(M - Mu), wc = fastExp2(m - Mu);  // (-inf: 0)
+                M = top;
+                L = fmaf(L, keep, wc * l);
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v].x *= keep, acc[v].y *= keep, acc[v].z *= keep, acc[v].w *= keep;
+                for (uint32_t c0 = 0; c0 < n; c0 += A) {
+#pragma unroll
+                    for (uint32_t u = 0; u < A; ++u) {
+                        if (c0 + u >= n) break;
+                        if (c0 > 0u) load(c0 + u, x[u]);
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < A; ++u) {
+                        if (c0 + u >= n) break;
+                        const float f = __shfl_sync(0xffffffffu, wc, c0 + u);
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            acc[v].x = fmaf(f, x[u][v].x, acc[v].x), acc[v].y = fmaf(f, x[u][v].y, acc[v].y);
+                            acc[v].z = fmaf(f, x[u][v].z, acc[v].z), acc[v].w = fmaf(f, x[u][v].w, acc[v].w);
+                        }
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
+            for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        }
+        if (W > 1u) {  // (the same for the whole block)
+            if (lane == 0) sMl[warp] = make_float2(M, L);
+#pragma unroll
+            for (int v = 0; v < V; ++v) sAcc[warp][v * 32 + lane] = acc[v];
+            __syncthreads();
+            if (mine == 0u) {
+                const float own = M;
+                for (uint32_t w = 1; w < W; ++w) M = fmaxf(M, sMl[warp + w].x);
+                const float Mu = M == -INFINITY ? 0.0f : M;
+                const float f0 = fastExp2(own - Mu);
+                L *= f0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v].x *= f0, acc[v].y *= f0, acc[v].z *= f0, acc[v].w *= f0;
+                for (uint32_t w = 1; w < W; ++w) {
+                    const float f = fastExp2(sMl[warp + w].x - Mu);
+                    L = fmaf(f, sMl[warp + w].y, L);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const float4 x = sAcc[warp + w][v * 32 + lane];
+                        acc[v].x = fmaf(f, x.x, acc[v].x), acc[v].y = fmaf(f, x.y, acc[v].y);
+                        acc[v].z = fmaf(f, x.z, acc[v].z), acc[v].w = fmaf(f, x.w, acc[v].w);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (mine != 0u || i >= rows) continue;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // (nothing seen)
 #pragma unroll
         for (int v = 0; v < V; ++v)
             if (HD >= 128 || lane < HD / 4u)
-                pagedStore<HD, MR>(p, w.s, w.kvHead, r, (v * 32u + lane) * 4u, make_float4(acc[v].x * inv, acc[v].y * inv, acc[v].z * inv, acc[v].w * inv));
+                pagedStore(p, HD, j.token0, j.kvHead, j.row0 + i, (v * 32u + lane) * 4u, make_float4(acc[v].x * inv, acc[v].y * inv, acc[v].z * inv, acc[v].w * inv));
     }
 }
 
@@ -160,8 +197,11 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     __syncthreads();
     gridDepWait();
     gridDepLaunch();
-    PagedWalk<MR> w;
-    if (!w.begin(p)) return;
+    PagedWalk w;
+    if (!w.begin(p, MR)) {
+        if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
+        return;
+    }
     bool ok = true;
     uint32_t g = 0;  // tiles so far
 
@@ -185,7 +225,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     }
                 }
                 const uint32_t st = g % NST;
-                if (g >= NST) ok = paWait(&empty[st], ((g / NST) - 1u) & 1u, p.c.err, kDevErrEmptyWait);
+                if (g >= NST) ok = pfWait<true>(&empty[st], ((g / NST) - 1u) & 1u, p.c.err, kDevErrEmptyWait);
                 if (!ok) break;
                 if (lane == 0) mbarExpectTx(&full[st], n * boxBytes * 2u * L::kPanels);
                 __syncwarp();
@@ -215,7 +255,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         } while (ok && w.next(p));
         // no copy is under way any more when the block leaves
         for (uint32_t back = 1; back <= NST && back <= g; ++back)
-            if (!paWait(&full[(g - back) % NST], ((g - back) / NST) & 1u, p.c.err, kDevErrFullWait)) break;
+            if (!pfWait<true>(&full[(g - back) % NST], ((g - back) / NST) & 1u, p.c.err, kDevErrFullWait)) break;
         return;
     }
 
@@ -230,7 +270,6 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const uint32_t key0 = wk * L::KS;
     float *buf = reinterpret_cast<float *>(smem + L::kBuf);
     float2 *ml = reinterpret_cast<float2 *>(smem + L::kMl);
-    volatile uint32_t *flag = reinterpret_cast<volatile uint32_t *>(smem + L::kFlag);
     auto groupSync = [&] {
         if (WK == 1) __syncwarp();
         else namedBarSync(1u + wm, WK * 32u);
@@ -302,7 +341,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         const uint32_t t0 = w.first(), t1 = w.last();
         for (uint32_t t = t0; t < t1; ++t, ++g) {
             const uint32_t st = g % NST;
-            ok = ok && paWait(&full[st], (g / NST) & 1u, p.c.err, kDevErrFullWait);
+            ok = ok && pfWait<true>(&full[st], (g / NST) & 1u, p.c.err, kDevErrFullWait);
             if (!ok) break;
             const uint32_t sK = smemAddr(smem + st * L::kStage), sV = sK + L::kMat;
             const float *sc = reinterpret_cast<const float *>(smem + L::kScales) + st * 128u;
@@ -538,26 +577,13 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 const uint32_t dim = I8 ? 128u * (pass / 4) + 16u * q4 + 4u * (pass % 4) : 32u * pass + 4u * q4;
                 const uint32_t local = wm * L::RW + row, r = w.item * MR + local;
                 if (r >= w.s.rows) continue;
-                if (whole) pagedStore<HD, MR>(p, w.s, w.kvHead, r, dim, x);
+                if (whole) pagedStore(p, HD, w.s.token0, w.kvHead, r, dim, x);
                 else __stcg(reinterpret_cast<float4 *>(part + local * HD + dim), x);
             }
         }
         groupSync();
-        if (!whole) {
-            __threadfence();
-            namedBarSync(6u, 128u);
-            if (threadIdx.x == 0) {
-                const uint32_t drawn = atomicAdd(&p.tickets[c0], 1u);
-                *flag = drawn == c1 - c0 ? 1u : 0u;
-                if (drawn == c1 - c0) p.tickets[c0] = 0u;
-            }
-            namedBarSync(6u, 128u);
-            if (*flag != 0u) {
-                __threadfence();
-                pagedMerge<HD, MR>(p, w, c0, c1 - c0 + 1u);
-            }
-            namedBarSync(6u, 128u);  // (the flag may be written again)
-        }
+        // (the last item of a block is the one that may go on in the next)
+        if (threadIdx.x == 0 && w.item0 + w.tiles >= w.end) pagedLeaveJoin(p, &w, !whole && blockIdx.x == c0 ? c1 - c0 + 1u : 0u);
     } while (w.next(p));
 }
 
@@ -572,7 +598,10 @@ static int launchPagedRows(const CUtensorMap &k, const CUtensorMap &v, const Pag
         TC_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
         attrDone[dev] = true;
     }
-    return launchDependent(kern, dim3(std::min(numSMs(), kPagedSMs) * L::kBlocks), kPaThreads, L::kTotal, st, 1, k, v, p);
+    const uint32_t blocks = std::min(numSMs(), kPagedSMs) * L::kBlocks;
+    const int rc = launchDependent(kern, dim3(blocks), kPaThreads, L::kTotal, st, 1, k, v, p);
+    if (rc != TC_OK) return rc;
+    return launchDependent(pagedMergeKernel<HD>, dim3(blocks, 8), 256, 0, st, 1, p);
 }
 
 int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v) {
@@ -642,7 +671,7 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
     p.c = pagedView(c, err);
     p.q = q, p.out = out, p.ks = c->ks, p.vs = c->vs;
     p.parts = static_cast<float *>(workspace);
-    p.tickets = reinterpret_cast<unsigned int *>(p.parts + kPagedParts);
+    p.joins = reinterpret_cast<PagedJoin *>(p.parts + kPagedParts);
     p.nHeads = nHeads, p.group = nHeads / c->nKV;
     p.box = 64;
     while (c->pageRows % p.box != 0) p.box /= 2;

@@ -4,7 +4,7 @@
 // r % group of its token r / group, so the heads that share K and V sit side by side and one pass over the rows serves them.  A
 // unit is one tile of kPaTile cache rows of an item.  The units of all items in a row -- sequence, kv head, rows -- are cut into
 // equal runs, one per block: ragged lengths, single tokens and prompts fill the SMs alike.  An item that lies in several runs
-// is put together by the block of it that finishes last, from partials in the workspace.
+// is put together by a second launch from partials in the workspace.
 #pragma once
 
 #include "paged.cuh"
@@ -13,13 +13,20 @@ namespace tc {
 
 constexpr uint32_t kPaTile = 64;  // cache rows of a unit
 
+// An item that lies in several blocks' runs, as the first of them leaves it for the merge: `count` blocks from this one on; their
+// partials are acc [mr][hd], m [mr], l [mr] (out = sum exp2(m - M) acc / sum exp2(m - M) l), in the first block's second slot -- its
+// run ends with the item -- and the others' first one.  count 0: nothing to join.
+struct PagedJoin {
+    uint32_t count, row0, rows, token0, kvHead, mr, pad[2];  // rows: of the sequence's kv head; row0: the item's first
+};
+
 struct PagedAttnParams {
     PagedView c;
     const void *q;   // [tokens][nHeads][hd] f32 / fp16
     void *out;
     const float *ks, *vs;
     float *parts;            // two slots per block
-    unsigned int *tickets;   // one per block, zero between launches
+    PagedJoin *joins;        // one per block
     uint32_t nHeads, group, box;  // box: cache rows of one TMA copy
     uint32_t minRows, maxRows;    // the kernel takes the sequences with so many query rows per kv head (minRows .. maxRows)
     float scaleLog2;
@@ -52,29 +59,25 @@ struct PagedSeq {
         const int32_t n = before + static_cast<int32_t>((end - 1u) / group) + 1;
         return n > 0 ? static_cast<uint32_t>(n) : 0u;
     }
-    template <uint32_t MR>
-    __device__ __forceinline__ uint32_t items() const { return (rows + MR - 1u) / MR; }
+    __device__ __forceinline__ uint32_t items(uint32_t MR) const { return (rows + MR - 1u) / MR; }
     // tiles of item m: one at least, which writes the zeros of rows that see nothing.  Where `before` is negative every item is
     // counted with the tiles of the whole sequence, so that the sum below keeps its closed form.
-    template <uint32_t MR>
-    __device__ __forceinline__ uint32_t tiles(uint32_t m, uint32_t group) const {
+    __device__ __forceinline__ uint32_t tiles(uint32_t MR, uint32_t m, uint32_t group) const {
         const uint32_t n = before < 0 ? len : sees(min((m + 1u) * MR, rows), group);
         return max(1u, (n + kPaTile - 1u) / kPaTile);
     }
     // tiles of items 0 .. m - 1
-    template <uint32_t MR>
-    __device__ __forceinline__ uint64_t tilesBefore(uint32_t m, uint32_t group) const {
+    __device__ __forceinline__ uint64_t tilesBefore(uint32_t MR, uint32_t m, uint32_t group) const {
         if (m == 0u) return 0u;
-        if (before < 0) return static_cast<uint64_t>(m) * tiles<MR>(0, group);
-        const bool all = m == items<MR>();
+        if (before < 0) return static_cast<uint64_t>(m) * tiles(MR, 0, group);
+        const bool all = m == items(MR);
         const uint32_t n = all ? m - 1u : m;
-        uint64_t sum = all ? tiles<MR>(m - 1u, group) : 0u;
+        uint64_t sum = all ? tiles(MR, m - 1u, group) : 0u;
         // item i sees before + ((i + 1) MR - 1) / group + 1 rows: floor((group (before + kPaTile) + (i + 1) MR - 1) / (kPaTile group)) tiles
         if (n > 0u) sum += floorSum(n, static_cast<uint64_t>(kPaTile) * group, MR, static_cast<uint64_t>(group) * (static_cast<uint32_t>(before) + kPaTile) + MR - 1u);
         return sum;
     }
-    template <uint32_t MR>
-    __device__ __forceinline__ uint64_t tilesAll(uint32_t group) const { return rows == 0u ? 0u : tilesBefore<MR>(items<MR>(), group); }
+    __device__ __forceinline__ uint64_t tilesAll(uint32_t MR, uint32_t group) const { return rows == 0u ? 0u : tilesBefore(MR, items(MR), group); }
 };
 
 __device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, uint32_t b) {
@@ -94,9 +97,9 @@ __device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, uint32_t 
     return s;
 }
 
-// A walk over a block's run of units, item by item; every warp makes its own, in step.  MR: query rows of an item.
-template <uint32_t MR>
+// A walk over a block's run of units, item by item; every warp makes its own, in step.
 struct PagedWalk {
+    uint32_t mr;              // query rows of an item
     uint64_t total, at, end;  // units of the launch; the block's next and last
     uint32_t blocks;          // blocks with work
     uint32_t seq, kvHead, item;
@@ -108,11 +111,12 @@ struct PagedWalk {
     __device__ __forceinline__ uint32_t blockOf(uint64_t unit) const { return static_cast<uint32_t>(((unit + 1u) * blocks - 1u) / total); }
 
     // All lanes of the warp.  False: nothing to do.
-    __device__ __forceinline__ bool begin(const PagedAttnParams &p) {
+    __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows) {
+        mr = itemRows;
         const uint32_t lane = threadIdx.x & 31u;
         uint64_t sum = 0;
         for (uint32_t b0 = 0; b0 < p.c.batch; b0 += 32u)
-            if (b0 + lane < p.c.batch) sum += pagedSeq(p, b0 + lane).template tilesAll<MR>(p.group) * p.c.nKV;
+            if (b0 + lane < p.c.batch) sum += pagedSeq(p, b0 + lane).tilesAll(mr, p.group) * p.c.nKV;
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum;
@@ -124,7 +128,7 @@ struct PagedWalk {
         uint64_t base = 0;
         for (uint32_t b0 = 0;; b0 += 32u) {
             uint64_t mine = 0;
-            if (b0 + lane < p.c.batch) mine = pagedSeq(p, b0 + lane).template tilesAll<MR>(p.group) * p.c.nKV;
+            if (b0 + lane < p.c.batch) mine = pagedSeq(p, b0 + lane).tilesAll(mr, p.group) * p.c.nKV;
             uint64_t upTo = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -142,18 +146,18 @@ struct PagedWalk {
             if (b0 + 32u >= p.c.batch) return false;  // (not reached: `at` lies below the sum)
         }
         s = pagedSeq(p, seq);
-        const uint64_t per = s.template tilesAll<MR>(p.group);
+        const uint64_t per = s.tilesAll(mr, p.group);
         kvHead = static_cast<uint32_t>((at - base) / per);
         const uint64_t in = at - base - kvHead * per;
-        uint32_t lo = 0, hi = s.template items<MR>() - 1u;  // the last item whose first tile is not behind `in`
+        uint32_t lo = 0, hi = s.items(mr) - 1u;  // the last item whose first tile is not behind `in`
         while (lo < hi) {
             const uint32_t mid = (lo + hi + 1u) / 2u;
-            if (s.template tilesBefore<MR>(mid, p.group) <= in) lo = mid;
+            if (s.tilesBefore(mr, mid, p.group) <= in) lo = mid;
             else hi = mid - 1u;
         }
         item = lo;
-        item0 = base + kvHead * per + s.template tilesBefore<MR>(item, p.group);
-        tiles = s.template tiles<MR>(item, p.group);
+        item0 = base + kvHead * per + s.tilesBefore(mr, item, p.group);
+        tiles = s.tiles(mr, item, p.group);
         return true;
     }
     // Tiles [first, last) of the item are the block's.
@@ -164,7 +168,7 @@ struct PagedWalk {
         item0 += tiles;
         at = item0;
         if (at >= end) return false;
-        if (++item == s.template items<MR>()) {
+        if (++item == s.items(mr)) {
             item = 0;
             if (++kvHead == p.c.nKV) {
                 kvHead = 0;
@@ -174,10 +178,17 @@ struct PagedWalk {
                 } while (s.rows == 0u);
             }
         }
-        tiles = s.template tiles<MR>(item, p.group);
+        tiles = s.tiles(mr, item, p.group);
         return true;
     }
 };
+// The block's entry for the merge; one thread, whether the block has work or not.
+__device__ __forceinline__ void pagedLeaveJoin(const PagedAttnParams &p, const PagedWalk *w, uint32_t count) {
+    PagedJoin j;
+    j.count = count;
+    if (count != 0u) j.row0 = w->item * w->mr, j.rows = w->s.rows, j.token0 = w->s.token0, j.kvHead = w->kvHead, j.mr = w->mr;
+    p.joins[blockIdx.x] = j;
+}
 #endif
 
 int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v);  // maps of the pools, `box` rows a copy

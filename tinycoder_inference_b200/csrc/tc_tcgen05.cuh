@@ -126,6 +126,51 @@ __device__ __forceinline__ void tmemSt16(uint32_t taddr, const uint32_t (&r)[16]
 }
 __device__ __forceinline__ void tmemStWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---- what the prefill kernels share ------------------------------------------------------------
+// Bounded wait: 2^18 polls, each parked for up to 20 us by the hardware.
+__device__ __forceinline__ bool pfPoll(uint64_t *bar, uint32_t parity, unsigned int *err, uint32_t bit) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 18); ++i) {
+        if (mbarTryWait(bar, parity)) return true;
+        // somebody has already given up: what this thread waits for will not come either
+        if ((i & 63u) == 63u &&
+            (*reinterpret_cast<volatile unsigned int *>(err) & (kDevErrFullWait | kDevErrEmptyWait | kDevErrMmaWait)) != 0u)
+            return false;
+    }
+    atomicOr(err, bit);
+    return false;
+}
+static __device__ __noinline__ bool pfPollCall(uint64_t *bar, uint32_t parity, unsigned int *err, uint32_t bit) {
+    return pfPoll(bar, parity, err, bit);
+}
+// Most waits find their phase complete, a step's chain goes through five of them, and their code sits in the middle of long
+// unrolled loops: the first poll stands alone and the loop behind it is a call.  Launch of 4096 rows of 28 / 4 / 128 (rows
+// launch included) 139.6 us with a loop that reads the clock, 135.3 with the first poll in front of a short loop,
+// 130.0 with that loop as a call; 512 rows behind 3584 49.7, 43.7 and 43.4.
+template <bool CALL>
+__device__ __forceinline__ bool pfWait(uint64_t *bar, uint32_t parity, unsigned int *err, uint32_t bit) {
+    return mbarTryWait(bar, parity) || (CALL ? pfPollCall(bar, parity, err, bit) : pfPoll(bar, parity, err, bit));
+}
+
+// one 32-byte store (the address has to be 32-byte aligned)
+__device__ __forceinline__ void stGlobalV8(float *dst, float a, float b, float c, float d, float e, float f, float g,
+                                           float h) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(a), "f"(b), "f"(c), "f"(d),
+                 "f"(e), "f"(f), "f"(g), "f"(h)
+                 : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// A matrix descriptor whose start address is moved by `bytes` (the address field holds
+// bytes >> 4 in its low 14 bits; shared memory is far smaller than their range, so the sum
+// never carries out of the field).
+__device__ __forceinline__ uint64_t descAdvance(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
+
 #endif  // __CUDACC__
 
 }  // namespace tc

@@ -288,7 +288,7 @@ def paged_workspace(device=None):
     """What attn_paged calls need, one for all calls that follow one another."""
     n = C.c_size_t(0)
     check(lib.tc_attn_paged_workspace_bytes(C.byref(n)))
-    return torch.zeros(n.value // 4, dtype=torch.float32, device=device or torch.device("cuda", torch.cuda.current_device()))
+    return torch.empty(n.value // 4, dtype=torch.float32, device=device or torch.device("cuda", torch.cuda.current_device()))
 
 
 def attn_paged(q, kc, vc, pages, lens, out, ws, starts=None, max_tokens=0, ks=None, vs=None, invSqrt=None):
