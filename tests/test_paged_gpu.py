@@ -148,6 +148,18 @@ def test_chunks(ws, store, nH, nKV, hd, io, lens, new, page):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("store,nH,nKV,hd", MODELS)
+@pytest.mark.parametrize("lens,new,page", [([300], [300], 16), ([1500, 1, 700, 64, 2000], [900, 1, 3, 64, 300], 32), ([3000], [128], 8),
+                                           ([40, 500], [90, 400], 16), ([1027, 900], [37, 19], 64), ([5000], [20], 48)])
+def test_chunks_of_many_rows(ws, store, nH, nKV, hd, lens, new, page):
+    """Whole prompts, chunks behind long prefixes, both beside single tokens, items of one and of two query tiles, runs that end
+    inside an item; more new tokens than rows."""
+    c = Paged(store, nH, nKV, hd, lens, new, page)
+    q = c.normal(c.tokens, nH, hd).half()
+    c.check(q, c.attend(q, ws, max(new)))
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("store,hd", [("f16", 64), ("f16", 128), ("f16", 256), ("i8", 128), ("i8", 256)])
 @pytest.mark.parametrize("seed", range(4))
 def test_random_batches(ws, store, hd, seed):

@@ -26,10 +26,11 @@
 namespace tc {
 
 constexpr int kPaThreads = 160;       // four consumer warps, one producer warp
-// The workspace: two partials per block of the widest grid, then what the merge finds per block.
-constexpr int kPagedSMs = 148;
-constexpr size_t kPagedParts = size_t(2) * kPagedSMs * 2 * 64 * (128 + 2);  // f32
-constexpr size_t kPagedWorkspace = kPagedParts * 4 + size_t(kPagedSMs) * 2 * sizeof(PagedJoin);
+// The workspace: two partials per block of the two kernels' widest grids, then what the merge finds per block.
+constexpr size_t kRowsParts = size_t(2) * kPagedSMs * 2 * pagedSlot(64, 128);       // f32
+constexpr size_t kTilesParts = size_t(2) * kPagedSMs * pagedSlot(2 * kPagedTile, 128);
+static_assert(2 * pagedSlot(64, 128) >= pagedSlot(64, 256) && pagedSlot(2 * kPagedTile, 128) >= pagedSlot(kPagedTile, 256), "one block per SM at head_dim 256");
+constexpr size_t kPagedWorkspace = (kRowsParts + kTilesParts) * 4 + size_t(kPagedSMs) * 3 * sizeof(PagedJoin) + 32;
 constexpr float kPaOff = 13.0f;       // p is held as 2^13 p: its fp16 pair keeps 11 + 11 bits down to p = 2^-27
 
 template <int HD, bool I8, bool PAIR, int WM>
@@ -77,17 +78,20 @@ __device__ __forceinline__ void pagedStore(const PagedAttnParams &p, uint32_t hd
 // W warps share a row, each a W-th of its partials: few rows of many parts (a step of one long session: 74) are as much a chain of loads
 // as many rows of two.
 template <int HD>
-__global__ void __launch_bounds__(256) pagedMergeKernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(256) pagedMergeKernel(const __grid_constant__ PagedAttnParams p, const float *partsB, const PagedJoin *joinsB, uint32_t blocksA) {
     constexpr int V = HD / 128 ? HD / 128 : 1;  // float4 of a lane
     __shared__ float4 sAcc[8][V * 32];
     __shared__ float2 sMl[8];
     gridDepWait();
     gridDepLaunch();
-    const PagedJoin j = p.joins[blockIdx.x];
+    const bool second = blockIdx.x >= blocksA;  // (the tiles kernel's)
+    const uint32_t from = second ? blockIdx.x - blocksA : blockIdx.x;
+    const PagedJoin j = (second ? joinsB : p.joins)[from];
     if (j.count == 0u) return;
+    const float *parts = second ? partsB : p.parts;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const size_t slot = static_cast<size_t>(j.mr) * (HD + 2);
-    auto part = [&](uint32_t c) { return p.parts + (2u * static_cast<size_t>(blockIdx.x + c) + (c == 0u ? 1u : 0u)) * slot; };
+    const size_t slot = pagedSlot(j.mr, HD);
+    auto part = [&](uint32_t c) { return parts + (2u * static_cast<size_t>(from + c) + (c == 0u ? 1u : 0u)) * slot; };
     const uint32_t W = j.count <= 8u ? 1u : j.count <= 16u ? 2u : j.count <= 32u ? 4u : 8u, perPass = 8u / W, mine = warp % W;
     const uint32_t rows = min(j.mr, j.rows - j.row0);
     for (uint32_t i0 = blockIdx.y * perPass; i0 < rows; i0 += gridDim.y * perPass) {
@@ -198,10 +202,8 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     gridDepWait();
     gridDepLaunch();
     PagedWalk w;
-    if (!w.begin(p, MR)) {
-        if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
-        return;
-    }
+    if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
+    if (!w.begin(p, MR)) return;
     bool ok = true;
     uint32_t g = 0;  // tiles so far
 
@@ -539,7 +541,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         }
         const bool whole = t0 == 0u && t1 == w.tiles;
         const uint32_t c0 = w.blockOf(w.item0), c1 = w.blockOf(w.item0 + w.tiles - 1u);
-        float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + (blockIdx.x == c0 ? 1u : 0u)) * (static_cast<size_t>(MR) * (HD + 2));
+        float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + (blockIdx.x == c0 ? 1u : 0u)) * pagedSlot(MR, HD);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const float Mu = M[r] == -INFINITY ? 0.0f : M[r];
@@ -582,11 +584,11 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             }
         }
         groupSync();
-        // (the last item of a block is the one that may go on in the next)
-        if (threadIdx.x == 0 && w.item0 + w.tiles >= w.end) pagedLeaveJoin(p, &w, !whole && blockIdx.x == c0 ? c1 - c0 + 1u : 0u);
+        if (threadIdx.x == 0 && !whole && blockIdx.x == c0) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
     } while (w.next(p));
 }
 
+static uint32_t pagedRowsBlocks(uint32_t hd) { return std::min(numSMs(), kPagedSMs) * (hd == 256 ? 1 : 2); }
 template <int HD, bool I8, bool PAIR, int WM>
 static int launchPagedRows(const CUtensorMap &k, const CUtensorMap &v, const PagedAttnParams &p, cudaStream_t st) {
     using L = PaL<HD, I8, PAIR, WM>;
@@ -598,10 +600,8 @@ static int launchPagedRows(const CUtensorMap &k, const CUtensorMap &v, const Pag
         TC_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
         attrDone[dev] = true;
     }
-    const uint32_t blocks = std::min(numSMs(), kPagedSMs) * L::kBlocks;
-    const int rc = launchDependent(kern, dim3(blocks), kPaThreads, L::kTotal, st, 1, k, v, p);
-    if (rc != TC_OK) return rc;
-    return launchDependent(pagedMergeKernel<HD>, dim3(blocks, 8), 256, 0, st, 1, p);
+    const uint32_t blocks = pagedRowsBlocks(HD);
+    return launchDependent(kern, dim3(blocks), kPaThreads, L::kTotal, st, 1, k, v, p);
 }
 
 int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v) {
@@ -638,6 +638,9 @@ static int pagedAttnRows(const tc_paged_kv *c, const PagedAttnParams &p, uint32_
 #undef TC_PAGED_WM
 }
 
+// Query rows per kv head from which on a call's sequences are tiles of the tensor cores; in such a call, what the rows kernel keeps.
+constexpr uint32_t kTilesFrom = 64, kRowsBeside = 16;
+
 }  // namespace tc
 
 extern "C" {
@@ -667,18 +670,43 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
     TC_REQUIRE(err != nullptr, TC_ECUDA, "no CUDA device");
     const uint32_t most = c->starts != nullptr ? c->tokens : c->tokens / c->batch;
     if (maxTokens == 0 || maxTokens > most) maxTokens = most;
+    const uintptr_t base = (reinterpret_cast<uintptr_t>(workspace) + 31) & ~uintptr_t(31);
     PagedAttnParams p;
     p.c = pagedView(c, err);
     p.q = q, p.out = out, p.ks = c->ks, p.vs = c->vs;
-    p.parts = static_cast<float *>(workspace);
-    p.joins = reinterpret_cast<PagedJoin *>(p.parts + kPagedParts);
+    p.parts = reinterpret_cast<float *>(base);
+    float *const partsB = p.parts + kRowsParts;
+    p.joins = reinterpret_cast<PagedJoin *>(partsB + kTilesParts);
+    PagedJoin *const joinsB = p.joins + 2 * kPagedSMs;
     p.nHeads = nHeads, p.group = nHeads / c->nKV;
     p.box = 64;
     while (c->pageRows % p.box != 0) p.box /= 2;
+    p.tileTokens = kPagedTile / p.group;
+    p.out32 = (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
     p.scaleLog2 = invSqrt * kLog2e;
     p.half = half != 0;
-    p.minRows = 1, p.maxRows = 0xffffffffu;
-    return pagedAttnRows(c, p, maxTokens * p.group, static_cast<cudaStream_t>(stream));
+    const uint32_t rows = maxTokens * p.group;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Sequences with many query rows go to the tensor cores' tiles, the others of the call to the rows kernel.
+    const bool tiles = half && !c->kvI8 && rows > kTilesFrom;
+    const bool rowsToo = !tiles || (c->starts != nullptr && c->batch > 1);
+    uint32_t blocksA = 0;
+    if (rowsToo) {
+        p.minRows = 1, p.maxRows = tiles ? kRowsBeside : 0xffffffffu;
+        const int ra = pagedAttnRows(c, p, tiles ? kRowsBeside : rows, st);
+        if (ra != TC_OK) return ra;
+        blocksA = pagedRowsBlocks(c->hd);
+    }
+    if (tiles) {
+        PagedAttnParams b = p;
+        b.parts = partsB, b.joins = joinsB;
+        b.minRows = rowsToo ? kRowsBeside + 1 : 1, b.maxRows = 0xffffffffu;
+        const int rb = pagedAttnTiles(c, b, st);
+        if (rb != TC_OK) return rb;
+    }
+    const dim3 grid(blocksA + (tiles ? std::min(numSMs(), kPagedSMs) : 0), 8);
+    auto merge = c->hd == 64 ? pagedMergeKernel<64> : c->hd == 128 ? pagedMergeKernel<128> : pagedMergeKernel<256>;
+    return launchDependent(merge, grid, 256, 0, st, 1, p, static_cast<const float *>(partsB), static_cast<const PagedJoin *>(joinsB), blocksA);
 }
 
 }  // extern "C"

@@ -16,6 +16,7 @@ constexpr uint32_t kPaTile = 64;  // cache rows of a unit
 // An item that lies in several blocks' runs, as the first of them leaves it for the merge: `count` blocks from this one on; their
 // partials are acc [mr][hd], m [mr], l [mr] (out = sum exp2(m - M) acc / sum exp2(m - M) l), in the first block's second slot -- its
 // run ends with the item -- and the others' first one.  count 0: nothing to join.
+__host__ __device__ constexpr size_t pagedSlot(uint32_t mr, uint32_t hd) { return (static_cast<size_t>(mr) * (hd + 2) + 7) & ~size_t(7); }  // f32
 struct PagedJoin {
     uint32_t count, row0, rows, token0, kvHead, mr, pad[2];  // rows: of the sequence's kv head; row0: the item's first
 };
@@ -28,6 +29,8 @@ struct PagedAttnParams {
     float *parts;            // two slots per block
     PagedJoin *joins;        // one per block
     uint32_t nHeads, group, box;  // box: cache rows of one TMA copy
+    uint32_t tileTokens;          // tiles kernel: tokens of a query tile
+    uint32_t out32;               // out is 32-byte aligned
     uint32_t minRows, maxRows;    // the kernel takes the sequences with so many query rows per kv head (minRows .. maxRows)
     float scaleLog2;
     int half;                // q and out are fp16
@@ -190,6 +193,11 @@ __device__ __forceinline__ void pagedLeaveJoin(const PagedAttnParams &p, const P
     p.joins[blockIdx.x] = j;
 }
 #endif
+
+// paged_tiles.cu: the sequences of minRows query rows per kv head and more, fp16 queries over an fp16 store, on tcgen05
+int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st);
+constexpr int kPagedSMs = 148;      // blocks that the workspace has room for, per block of an SM
+constexpr uint32_t kPagedTile = 128;  // query rows of a tile of the tiles kernel
 
 int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v);  // maps of the pools, `box` rows a copy
 

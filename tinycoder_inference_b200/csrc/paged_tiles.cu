@@ -1,0 +1,529 @@
+// paged_tiles.cu -- attention of many query rows per kv head over an fp16 paged cache on tcgen05 (fp16 queries and results, f32
+// accumulation in TMEM): chunks of prompts and whole prompts.
+//
+// The block is prefill_f16.cu's: two 128-row query tiles A and B share a ring of 64-row K and V tiles, warps 0-3 / 4-7 hold the softmax of
+// A / B a thread per row, warp 8 requests, warps 9, 10 issue S = Q K^T and warps 11, 12 O += P V with P in TMEM over the scores' buffer.
+// What differs is what a tile is and where it comes from:
+//   * a query tile holds tileTokens tokens x the q heads of one kv head (row = token x group + head; one TMA box), so a
+//     pass over the cache serves all of them and the causal edge is tileTokens rows wide instead of 128;
+//   * K and V tiles are gathered page by page, a TMA copy per `box` rows, issued by the lanes of the producer warp side by side;
+//   * the work is the runs of paged_attn.cuh: a block's run of tiles may begin and end inside an item, whose partials the
+//     merge launch joins.  An item of one query tile gives its KV tiles to the two halves in turn (even / odd);
+//   * rows past the sequence may hold anything: scores there are masked by selects, and the warp that issues P V writes zeros over V's.
+#include <cstring>
+
+#include "paged_attn.cuh"
+#include "tc_tcgen05.cuh"
+
+namespace tc {
+
+constexpr int kPtThreads = 416;
+constexpr int kPtBN = int(kPaTile);
+constexpr float kPtLazyLog2 = 8.0f;  // O is rescaled when the row's maximum ran ahead by 2^8
+
+template <int HD>
+struct PtL {
+    static constexpr int kHalves = HD / 64;
+    static constexpr int kQTiles = HD > 128 ? 1 : 2;
+    static constexpr int NK = HD > 128 ? 2 : 6, NV = HD > 128 ? 2 : 4;
+    static constexpr int kQHalf = int(kPagedTile) * 128;
+    static constexpr int kKvHalf = kPtBN * 128;
+    static constexpr int kQTile = kHalves * kQHalf;
+    static constexpr int kKvTile = kHalves * kKvHalf;
+    static constexpr int kQ = 0;
+    static constexpr int kK = kQTiles * kQTile;
+    static constexpr int kV = kK + NK * kKvTile;
+    static constexpr int kExch = kV + NV * kKvTile;  // [half][row] (m, l) of items of one tile
+    static constexpr int kBars = kExch + (HD > 128 ? 0 : 2 * int(kPagedTile) * 8);
+    // qFull, kFull + kEmpty, vFull + vEmpty, sFull[2][2], pFull[2][2], pvBuf[2][2], qFree[2], exFull, exRead, sFree[2]
+    static constexpr int kNumBars = 1 + 2 * NK + 2 * NV + 4 + 4 + 4 + 2 + 2 + 2;
+    static constexpr int kTmemSlot = kBars + kNumBars * 8;
+    static constexpr int kTotal = kTmemSlot + 16;
+    static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
+};
+
+// What a block has of an item: tiles j = 0 .. nTiles - 1 are cache rows 64 (t0 + j) ..; query tile X takes tile j if mine(X, j).
+struct PtItem {
+    uint32_t m0, rowsA, rowsB, t0, nTiles, nA, nB;
+    bool split, whole;
+    __device__ __forceinline__ bool mine(uint32_t x, uint32_t j) const { return split ? (j & 1u) == x : j < (x == 0u ? nA : nB); }
+};
+template <bool ONE>
+__device__ __forceinline__ PtItem ptItem(const PagedAttnParams &p, const PagedWalk &w) {
+    PtItem it;
+    const uint32_t tile = p.tileTokens * p.group;
+    it.m0 = w.item * w.mr;
+    const uint32_t rows = min(w.mr, w.s.rows - it.m0);
+    it.rowsA = min(rows, tile), it.rowsB = rows - it.rowsA;
+    it.t0 = w.first();
+    const uint32_t t1 = w.last();
+    it.nTiles = t1 - it.t0;
+    it.whole = it.t0 == 0u && t1 == w.tiles;
+    it.split = !ONE && it.rowsB == 0u;
+    if (it.split) {
+        it.nB = it.nTiles / 2u, it.nA = it.nTiles - it.nB;
+    } else {
+        // A's rows end before B's
+        const uint32_t tilesA = it.rowsB == 0u ? w.tiles : min(w.tiles, max(1u, (w.s.sees(it.m0 + it.rowsA, p.group) + kPaTile - 1u) / kPaTile));
+        it.nA = min(t1, tilesA) > it.t0 ? min(t1, tilesA) - it.t0 : 0u;
+        it.nB = it.rowsB != 0u ? it.nTiles : 0u;
+    }
+    return it;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPtThreads, 1)
+pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ PagedAttnParams p) {
+    using L = PtL<HD>;
+    constexpr int NC = kPtBN / 32;  // 32-column chunks of a score row
+    constexpr uint32_t NK = L::NK, NV = L::NV, BN = kPtBN;
+    constexpr bool kCall = HD < 256;
+    constexpr bool kOne = L::kQTiles == 1;
+    constexpr bool kAhead = kOne;   // one score buffer and two for probabilities (prefill_f16.cu)
+    extern __shared__ __align__(1024) uint8_t smem[];  // (head_dim 128 has no room to round the address up)
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
+    uint64_t *qFull = bars, *kFull = bars + 1, *kEmpty = kFull + NK, *vFull = kEmpty + NK, *vEmpty = vFull + NV, *sFull = vEmpty + NV /* [x][b] */,
+             *pFull = sFull + 4 /* [x][b] */, *pvBuf = pFull + 4 /* [x][b] */, *qFree = pvBuf + 4 /* [x] */,
+             *exFull = qFree + 2, *exRead = exFull + 1, *sFree = exRead + 1 /* [x] */;
+    uint32_t *tmemSlot = reinterpret_cast<uint32_t *>(smem + L::kTmemSlot);
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
+    unsigned int *const err = p.c.err;
+
+    if ((smemAddr(smem) & 1023u) != 0u) {  // the swizzle needs it; reported like the other resource that a block may not get
+        if (threadIdx.x == 0) {
+            gridDepWait();
+            pagedLeaveJoin(p, nullptr, 0u);
+            atomicOr(err, kDevErrTmemAlloc);
+        }
+        return;
+    }
+    if (threadIdx.x == 0) {
+        mbarInit(qFull, 1);
+        const uint32_t users = kOne ? 1u : 2u;  // a K (V) tile is released by the score (P.V) warps of both query tiles
+        for (uint32_t s = 0; s < NK; ++s) mbarInit(&kFull[s], 1), mbarInit(&kEmpty[s], users);
+        for (uint32_t s = 0; s < NV; ++s) mbarInit(&vFull[s], 1), mbarInit(&vEmpty[s], users);
+        for (int i = 0; i < 4; ++i) {
+            mbarInit(&sFull[i], 1);
+            mbarInit(&pFull[i], 4);  // one arrival per warp
+            mbarInit(&pvBuf[i], 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbarInit(&sFree[x], 4);
+            mbarInit(&qFree[x], 1);
+        }
+        mbarInit(exFull, 2 * kPagedTile);
+        mbarInit(exRead, 2 * kPagedTile);
+        fenceBarrierInit();
+        tmaPrefetchDesc(&tmQ);
+        tmaPrefetchDesc(&tmK);
+        tmaPrefetchDesc(&tmV);
+    }
+    if (warp == 0) {
+        tmemAlloc(tmemSlot, 512);
+        tmemRelinquish();
+        tcFenceBefore();
+    }
+    __syncthreads();
+    tcFenceAfter();
+    const uint32_t tmemBase = *reinterpret_cast<volatile uint32_t *>(tmemSlot);
+    gridDepWait();
+    gridDepLaunch();
+    const uint32_t tileRows = p.tileTokens * p.group;
+    if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
+    PagedWalk w;
+    const bool work = w.begin(p, tileRows * L::kQTiles);
+
+    if (!work) {
+    } else if (warp == 8) {
+        // ------------------------------- producer -------------------------------
+        uint32_t gk = 0, gv = 0, n = 0;
+        bool ok = true;
+        const uint32_t boxes = BN / p.box, boxBytes = p.box * 128u;
+        do {
+            const PtItem it = ptItem<kOne>(p, w);
+            const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
+            auto request = [&](uint32_t j, const CUtensorMap *map, uint32_t base, uint64_t *full, uint64_t *empty, uint32_t &g, uint32_t N) {
+                const uint32_t row0 = (it.t0 + j) * BN;
+                const uint32_t have = w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u;
+                uint32_t page = 0, in = 0;
+                if (lane < have) {
+                    const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
+                    in = row - slot * p.c.pageRows;
+                    page = static_cast<uint32_t>(__ldg(table + slot));
+                    if (page >= p.c.numPages) {  // no such page: reported, page 0 stands in
+                        atomicOr(err, kDevErrRowBound);
+                        page = 0;
+                    }
+                }
+                const uint32_t s = g % N;
+                if (g >= N && !pfWait<kCall>(&empty[s], ((g / N) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
+                if (lane == 0) mbarExpectTx(&full[s], have * boxBytes * L::kHalves);
+                __syncwarp();
+                if (lane < have) {
+#pragma unroll
+                    for (int h = 0; h < L::kHalves; ++h)
+                        tmaLoad4D(smem + base + s * L::kKvTile + h * L::kKvHalf + lane * boxBytes, map, &full[s], 64 * h, w.kvHead, in, page);
+                }
+                ++g;
+                return true;
+            };
+            auto requestK = [&](uint32_t j) { return request(j, &tmK, L::kK, kFull, kEmpty, gk, NK); };
+            auto requestV = [&](uint32_t j) { return request(j, &tmV, L::kV, vFull, vEmpty, gv, NV); };
+            // the query tiles are free once the last score products of the previous item are complete
+            if (n > 0)
+                ok = pfWait<kCall>(&qFree[0], (n - 1u) & 1u, err, kDevErrEmptyWait) && (kOne || pfWait<kCall>(&qFree[1], (n - 1u) & 1u, err, kDevErrEmptyWait));
+            if (!ok) break;
+            if (lane == 0) {
+                const uint32_t qTiles = it.rowsB != 0u ? 2u : 1u;
+                mbarExpectTx(qFull, qTiles * L::kHalves * tileRows * 128u);
+                for (uint32_t x = 0; x < qTiles; ++x)
+#pragma unroll
+                    for (int h = 0; h < L::kHalves; ++h)
+                        tmaLoad3D(smem + L::kQ + x * L::kQTile + h * L::kQHalf, &tmQ, qFull, 64 * h, w.kvHead * p.group,
+                                  w.s.token0 + it.m0 / p.group + x * p.tileTokens);
+            }
+            __syncwarp();
+            ok = requestK(0) && (it.nTiles < 2u || requestK(1));
+            for (uint32_t j = 0; ok && j < it.nTiles; ++j) ok = (j + 2u >= it.nTiles || requestK(j + 2u)) && requestV(j);
+            ++n;
+        } while (ok && w.next(p));
+        // the last release of every slot has to have arrived before the block leaves
+        for (uint32_t back = 1; ok && back <= NK && back <= gk; ++back) ok = pfWait<kCall>(&kEmpty[(gk - back) % NK], ((gk - back) / NK) & 1u, err, kDevErrEmptyWait);
+        for (uint32_t back = 1; ok && back <= NV && back <= gv; ++back) ok = pfWait<kCall>(&vEmpty[(gv - back) % NV], ((gv - back) / NV) & 1u, err, kDevErrEmptyWait);
+        if (!ok) {  // somebody gave up: the copies under way still land before the block leaves
+            for (uint32_t back = 1; back <= NK && back <= gk; ++back) pfWait<kCall>(&kFull[(gk - back) % NK], ((gk - back) / NK) & 1u, err, kDevErrFullWait);
+            for (uint32_t back = 1; back <= NV && back <= gv; ++back) pfWait<kCall>(&vFull[(gv - back) % NV], ((gv - back) / NV) & 1u, err, kDevErrFullWait);
+        }
+    } else if (warp >= 9) {
+        // ------------------------------- MMA issuers -------------------------------
+        // t counts the tiles of X over all items; tile t uses score buffer t % 2, which P(t - 2) has to have left (kAhead: the softmax
+        // threads have to have read S(t - 1)).  A tile that is not X's is released all the same, once it is there: a warp that ran ahead would
+        // hand in the release of a later round.
+        const uint32_t x = (warp - 9u) & 1u;
+        const bool pvRole = warp >= 11u;
+        constexpr uint32_t idQK = umaInstrDescF16(kPagedTile, BN, 0, 0);
+        constexpr uint32_t idPV = umaInstrDescF16(kPagedTile, HD, 0, 1);
+        const uint64_t dQ0 = umaSmemDesc(smemAddr(smem + L::kQ), 16, 1024);
+        const uint64_t dK0 = umaSmemDesc(smemAddr(smem + L::kK), 16, 1024);
+        const uint64_t dV0 = umaSmemDesc(smemAddr(smem + L::kV), L::kKvHalf, 1024);
+        const uint32_t tO = tmemBase + 128u * x, tS0 = tmemBase + 256u + 128u * x;
+        uint32_t g = 0, t = 0, n = 0;
+        bool ok = true;
+        if (!(kOne && x == 1u)) do {
+            const PtItem it = ptItem<kOne>(p, w);
+            const uint32_t myTiles = x == 0 ? it.nA : it.nB;
+            const uint64_t dQ = descAdvance(dQ0, it.split ? 0u : x * L::kQTile);
+            uint32_t tt = t;
+            for (uint32_t j = 0; ok && j < it.nTiles; ++j) {
+                const uint32_t gg = g + j;
+                const bool mine = it.mine(x, j);
+                if (!pvRole) {
+                    const uint32_t s = gg % NK;
+                    if (mine && tt == t) ok = pfWait<kCall>(qFull, n & 1u, err, kDevErrFullWait);
+                    ok = ok && pfWait<kCall>(&kFull[s], (gg / NK) & 1u, err, kDevErrFullWait);
+                    if (mine) {
+                        if (kAhead) {
+                            if (ok && tt >= 1u) ok = pfWait<kCall>(&sFree[x], (tt - 1u) & 1u, err, kDevErrMmaWait);
+                        } else if (ok && tt >= 2u) {
+                            ok = pfWait<kCall>(&pvBuf[2u * x + (tt & 1u)], ((tt - 2u) >> 1) & 1u, err, kDevErrMmaWait);
+                        }
+                        if (!ok) break;
+                        tcFenceAfter();
+                        const uint64_t dK = descAdvance(dK0, s * L::kKvTile);
+                        if (electOne()) {
+#pragma unroll
+                            for (uint32_t ks = 0; ks < HD / 16; ++ks)
+                                umaMmaSS(tS0 + (kAhead ? 0u : 64u * (tt & 1u)), descAdvance(dQ, (ks >> 2) * L::kQHalf + (ks & 3u) * 32u),
+                                         descAdvance(dK, (ks >> 2) * L::kKvHalf + (ks & 3u) * 32u), idQK, ks > 0 ? 1u : 0u);
+                            umaCommit(&sFull[kAhead ? x : 2u * x + (tt & 1u)]);
+                            if (tt + 1u == t + myTiles) umaCommit(&qFree[x]);
+                            umaCommit(&kEmpty[s]);
+                        }
+                        ++tt;
+                    } else if (ok && electOne()) {
+                        umaCommit(&kEmpty[s]);
+                    }
+                    __syncwarp();
+                } else {
+                    const uint32_t s = gg % NV;
+                    ok = pfWait<kCall>(&vFull[s], (gg / NV) & 1u, err, kDevErrFullWait);
+                    if (mine) {
+                        const uint32_t row0 = (it.t0 + j) * BN;
+                        if (ok && row0 + BN > w.s.len) {
+                            // rows past the sequence: zeros, whatever the pages (or an earlier tile) left there
+                            const uint32_t keep = w.s.len > row0 ? w.s.len - row0 : 0u;
+                            const uint32_t base = smemAddr(smem + L::kV + s * L::kKvTile);
+                            for (uint32_t i = lane; i < (BN - keep) * 8u * L::kHalves; i += 32u) {
+                                const uint32_t chunk = i & 7u, row = keep + (i >> 3) % (BN - keep), h = (i >> 3) / (BN - keep);
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + h * L::kKvHalf + row * 128u + chunk * 16u), "r"(0u) : "memory");
+                            }
+                            fenceProxyAsync();
+                            __syncwarp();
+                        }
+                        ok = ok && pfWait<kCall>(&pFull[2u * x + (tt & 1u)], (tt >> 1) & 1u, err, kDevErrMmaWait);
+                        if (!ok) break;
+                        tcFenceAfter();
+                        const uint64_t dV = descAdvance(dV0, s * L::kKvTile);
+                        const uint32_t tP = tS0 + (kAhead ? 64u + 32u * (tt & 1u) : 64u * (tt & 1u));
+                        if (electOne()) {
+#pragma unroll
+                            for (uint32_t ks = 0; ks < BN / 16; ++ks)  // 16 rows per step: 8 columns of fp16 P, 2 KB of V
+                                umaMmaTS(tO, tP + ks * 8u, descAdvance(dV, ks * 2048u), idPV, (tt > t || ks > 0) ? 1u : 0u);
+                            umaCommit(&pvBuf[2u * x + (tt & 1u)]);
+                            umaCommit(&vEmpty[s]);
+                        }
+                        ++tt;
+                    } else if (ok && electOne()) {
+                        umaCommit(&vEmpty[s]);
+                    }
+                    __syncwarp();
+                }
+            }
+            // A half without tiles hands in its phase of qFree, too, behind the item's last K tile and the query tiles (a
+            // parity wait cannot tell a phase that it skipped from the one before).
+            if (!pvRole && myTiles == 0u && ok) {
+                ok = pfWait<kCall>(qFull, n & 1u, err, kDevErrFullWait);
+                if (ok && electOne()) umaCommit(&qFree[x]);
+                __syncwarp();
+            }
+            t += myTiles;
+            g += it.nTiles;
+            ++n;
+        } while (ok && w.next(p));
+        if (pvRole && ok) {
+            // the last two buffer commits have to land before the block leaves
+            for (uint32_t tt = t >= 2u ? t - 2u : 0u; tt < t; ++tt)
+                if (!pfWait<kCall>(&pvBuf[2u * x + (tt & 1u)], (tt >> 1) & 1u, err, kDevErrMmaWait)) break;
+        }
+    } else if (!(kOne && warp >= 4)) {
+        // --------------------------------- softmax ---------------------------------
+        const uint32_t x = warp >> 2;                         // which query tile this warpgroup owns
+        const uint32_t row = (warp & 3u) * 32u + lane;        // row of that tile = TMEM lane
+        const uint32_t laneBase = ((warp & 3u) * 32u) << 16;  // TMEM lane field
+        const uint32_t tO = tmemBase + 128u * x;
+        float2 *exch = reinterpret_cast<float2 *>(smem + L::kExch);
+        uint32_t t = 0, nSplit = 0;  // tiles of X, items of one tile so far
+        bool ok = true;
+        do {
+            const PtItem it = ptItem<kOne>(p, w);
+            const uint32_t myTiles = x == 0 ? it.nA : it.nB;
+            const uint32_t myRows = it.split || x == 0u ? it.rowsA : it.rowsB;
+            const uint32_t c0 = w.blockOf(w.item0), c1 = w.blockOf(w.item0 + w.tiles - 1u);
+            if (threadIdx.x == 0 && !it.whole && blockIdx.x == c0) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
+            if (myRows == 0u) continue;  // (no query tile B)
+            const uint32_t tileRow0 = it.split ? 0u : x * tileRows;          // the tile's first row inside the item
+            const uint32_t rr = it.m0 + tileRow0 + row, tok = rr / p.group;  // row and token of the sequence
+            const int32_t pos = w.s.before + static_cast<int32_t>(tok);      // the last cache row that the query row sees
+            const int32_t pos0 = w.s.before + static_cast<int32_t>((it.m0 + tileRow0) / p.group);  // ... that the tile's first row does
+            float m = kNegBig, l = 0.0f;
+            for (uint32_t j = 0; j < myTiles; ++j) {
+                const uint32_t tt = t + j, b = tt & 1u;
+                const int32_t kt = static_cast<int32_t>(it.t0 + (it.split ? 2u * j + x : j));  // KV tile
+                const uint32_t tS = tmemBase + 256u + 128u * x + (kAhead ? 0u : 64u * b), tP = kAhead ? tS + 64u + 32u * b : tS;
+                if (!pfWait<kCall>(&sFull[kAhead ? x : 2u * x + b], (kAhead ? tt : tt >> 1) & 1u, err, kDevErrMmaWait)) {
+                    ok = false;
+                    break;
+                }
+                tcFenceAfter();
+                uint32_t r[NC][32];  // the scores of this row
+#pragma unroll
+                for (int c = 0; c < NC; ++c) tmemLd32(tS + laneBase + 32u * c, r[c]);
+                tmemLdWait();
+                if (kAhead) {
+                    tcFenceBefore();
+                    __syncwarp();
+                    if (lane == 0) mbarArrive(&sFree[x]);
+                }
+                if (kPtBN * kt + (kPtBN - 1) > pos0) {  // causal edge
+                    const int32_t first = kPtBN * kt - pos;
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (first + c * 32 + i > 0) r[c][i] = 0xff800000u;  // -inf
+                }
+                float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            mxs[u] = max3(mxs[u], __uint_as_float(r[c][i + 2 * u]), __uint_as_float(r[c][i + 2 * u + 1]));
+                const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * p.scaleLog2;  // scale > 0: max commutes with it
+                const float mNew = mx > m + kPtLazyLog2 ? mx : m;
+                const bool rescale = j > 0 && __any_sync(0xffffffffu, mNew != m);
+                float alpha = 1.0f;
+                // The products of tile t - 2 are complete: its probabilities' buffer may be written, and a wait for tile t - 1 below
+                // cannot take an older phase of its barrier for the one it means (a parity wait tells the current phase from the one
+                // before it only).  Without kAhead the score product of this tile has waited for them.
+                if (kAhead) {
+                    if (tt >= 2u && !pfWait<kCall>(&pvBuf[2u * x + b], ((tt - 2u) >> 1) & 1u, err, kDevErrMmaWait)) {
+                        ok = false;
+                        break;
+                    }
+                    tcFenceAfter();
+                }
+                if (rescale) {
+                    // O may only be touched between two of its P.V products
+                    if (!pfWait<kCall>(&pvBuf[2u * x + (b ^ 1u)], ((tt - 1u) >> 1) & 1u, err, kDevErrMmaWait)) {
+                        ok = false;
+                        break;
+                    }
+                    tcFenceAfter();
+                    alpha = fastExp2(m - mNew);
+#pragma unroll 1
+                    for (uint32_t c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tmemLd32(tO + laneBase + c * 32u, o);
+                        tmemLdWait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmemSt32(tO + laneBase + c * 32u, o);
+                    }
+                    tmemStWait();
+                }
+                m = mNew;
+                const float2 scale2 = make_float2(p.scaleLog2, p.scaleLog2), negM2 = make_float2(-m, -m);
+                float psum = 0.0f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    uint32_t h[16];
+                    float2 sum2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 x2 = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, negM2);
+                        const float2 p2 = make_float2(fastExp2(x2.x), fastExp2(x2.y));
+                        sum2 = __fadd2_rn(sum2, p2);
+                        h[i] = packHalf2(p2.x, p2.y);
+                    }
+                    psum += sum2.x + sum2.y;
+                    tmemSt16(tP + laneBase + c * 16u, h);
+                }
+                l = l * alpha + psum;
+                tmemStWait();
+                tcFenceBefore();
+                __syncwarp();
+                if (lane == 0) mbarArrive(&pFull[2u * x + b]);
+            }
+            if (myTiles != 0u) {
+                const uint32_t tt = t + myTiles - 1u;
+                ok = ok && pfWait<kCall>(&pvBuf[2u * x + (tt & 1u)], (tt >> 1) & 1u, err, kDevErrMmaWait);
+            }
+            if (!ok) break;
+            // Items of one query tile: each half leaves (m, l) of its rows for the other one and stores half of the dims, out of both
+            // accumulators (they lie in the same TMEM lanes).
+            float M = m, lAll = l, wMine = 1.0f, wOther = 0.0f;
+            if (it.split) {
+                exch[x * kPagedTile + row] = make_float2(m, l);
+                tcFenceBefore();
+                mbarArrive(exFull);
+                ok = pfWait<kCall>(exFull, nSplit & 1u, err, kDevErrMmaWait);
+                if (!ok) break;
+                tcFenceAfter();
+                const float2 o = exch[(x ^ 1u) * kPagedTile + row];
+                M = fmaxf(m, o.x), wMine = fastExp2(m - M), wOther = fastExp2(o.x - M);
+                lAll = fmaf(wMine, l, wOther * o.y);
+            } else {
+                tcFenceAfter();
+            }
+            const bool other = it.split && (x == 0u ? it.nB : it.nA) != 0u, own = myTiles != 0u;  // accumulators that were written
+            const float inv = it.whole ? (lAll == 0.0f ? 0.0f : 1.0f / lAll) : 1.0f;
+            wMine *= inv, wOther *= inv;
+            constexpr uint32_t kChunks = HD / 32;
+            const uint32_t k0 = it.split ? x * (kChunks / 2) : 0u, k1 = it.split ? k0 + kChunks / 2 : kChunks;
+            const uint32_t local = tileRow0 + row;  // row of the item
+            float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + (blockIdx.x == c0 ? 1u : 0u)) * pagedSlot(w.mr, HD);
+            if (!it.whole && row < myRows && (!it.split || x == 0u)) part[w.mr * HD + local] = M, part[w.mr * HD + w.mr + local] = lAll;
+            __half *orow = static_cast<__half *>(p.out) + (static_cast<size_t>(w.s.token0 + tok) * p.nHeads + w.kvHead * p.group + (rr - tok * p.group)) * HD;
+#pragma unroll 1
+            for (uint32_t c = k0; c < k1; ++c) {
+                uint32_t o[32];
+                if (own) {
+                    tmemLd32(tO + laneBase + c * 32u, o);
+                    tmemLdWait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * wMine);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0u;
+                }
+                if (other) {
+                    uint32_t o2[32];
+                    tmemLd32(tmemBase + 128u * (x ^ 1u) + laneBase + c * 32u, o2);
+                    tmemLdWait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), wOther, __uint_as_float(o[i])));
+                }
+                if (row < myRows && !it.whole) {
+                    // 32 bytes per store: a thread owns its row
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        stGlobalV8(part + static_cast<size_t>(local) * HD + c * 32 + 8 * i, __uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]),
+                                   __uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]), __uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]),
+                                   __uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
+                } else if (row < myRows) {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) h[i] = packHalf2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {
+                        if (!p.out32) {
+                            *reinterpret_cast<uint4 *>(orow + c * 32 + 2 * i) = make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+                            *reinterpret_cast<uint4 *>(orow + c * 32 + 2 * i + 8) = make_uint4(h[i + 4], h[i + 5], h[i + 6], h[i + 7]);
+                            continue;
+                        }
+                        stGlobalV8(reinterpret_cast<float *>(orow + c * 32 + 2 * i), __uint_as_float(h[i]), __uint_as_float(h[i + 1]), __uint_as_float(h[i + 2]),
+                                   __uint_as_float(h[i + 3]), __uint_as_float(h[i + 4]), __uint_as_float(h[i + 5]), __uint_as_float(h[i + 6]), __uint_as_float(h[i + 7]));
+                    }
+                }
+            }
+            if (it.split) {
+                // the next item's first P.V product may overwrite an accumulator once both halves have read it
+                tcFenceBefore();
+                mbarArrive(exRead);
+                ok = pfWait<kCall>(exRead, nSplit & 1u, err, kDevErrMmaWait);
+                ++nSplit;
+            } else {
+                tcFenceBefore();
+            }
+            t += myTiles;
+        } while (ok && w.next(p));
+    }
+    __syncthreads();
+    if (warp == 0) tmemDealloc(tmemBase, 512);
+}
+
+template <int HD>
+static int launchTiles(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const PagedAttnParams &p, cudaStream_t st) {
+    using L = PtL<HD>;
+    static bool attrDone[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !attrDone[dev]) {
+        TC_CUDA_OK(cudaFuncSetAttribute(pagedTilesKernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
+        attrDone[dev] = true;
+    }
+    return launchDependent(pagedTilesKernel<HD>, dim3(numSMs() < kPagedSMs ? numSMs() : kPagedSMs), kPtThreads, L::kTotal, st, 1, q, k, v, p);
+}
+
+int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st) {
+    CUtensorMap q, k, v;
+    int rc = pagedMaps(c, p.box, &k, &v);
+    if (rc != TC_OK) return rc;
+    TensorMapKey key;
+    memset(&key, 0, sizeof(key));
+    key.base = p.q;
+    key.dims[0] = c->hd, key.dims[1] = p.nHeads, key.dims[2] = c->tokens;
+    key.strides[0] = static_cast<uint64_t>(c->hd) * 2;
+    key.strides[1] = key.strides[0] * p.nHeads;
+    key.box[0] = 64, key.box[1] = p.group, key.box[2] = p.tileTokens;
+    key.rank = 3, key.elemBytes = 2, key.swizzle = 3;
+    rc = getTensorMap(key, &q);
+    if (rc != TC_OK) return rc;
+    if (c->hd == 64) return launchTiles<64>(q, k, v, p, st);
+    return c->hd == 128 ? launchTiles<128>(q, k, v, p, st) : launchTiles<256>(q, k, v, p, st);
+}
+
+}  // namespace tc
