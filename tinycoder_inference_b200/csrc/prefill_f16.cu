@@ -657,6 +657,10 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         float2 *exch = reinterpret_cast<float2 *>(smem + L::kQ + (kOne ? 0 : L::kQTile));
         uint32_t t = 0, item = 0;  // tiles of X done over all items
         bool ok = true;
+        auto pvWait = [&](uint32_t tile) {  // the P.V product of that tile is complete
+            return kAhead ? pfWait<kCall>(&pvBuf[2u * x + (tile & 1u)], (tile >> 1) & 1u, p.err, kDevErrMmaWait)
+                          : pfWait<kCall>(&pvDone[x], tile & 1u, p.err, kDevErrMmaWait);
+        };
         for (uint32_t n = 0; ok && takeItem(n, item); ++n) {
             const PfItem it = pfItem<SHARED>(p, item);
             const uint32_t m0 = it.m0, head = it.head;
@@ -711,13 +715,23 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const bool rescale = j > 0 && __any_sync(0xffffffffu, mNew != m);
                 float alpha = 1.0f;  // (without a rescale m stays: l is 0 in the first step)
                 if (row == 0 && x == 0) PF_STAMP(6u, j, 1);
+                if (kAhead) {
+                    // The products of tile t - 2 are complete: the buffer of their probabilities may be written, and the waits for the
+                    // previous tile below, which go by the same barriers, cannot take an older phase for the one they mean.  (Nothing else
+                    // holds the scores back until then: behind late V tiles they run two tiles and more ahead of the products.)
+                    if (tt >= 2u && !pfWait<kCall>(&pvBuf[2u * x + b], ((tt - 2u) >> 1) & 1u, p.err, kDevErrMmaWait)) {
+                        ok = false;
+                        break;
+                    }
+                    tcFenceAfter();
+                }
                 // O may only be touched between two of its PV products: the previous one has to be
                 // complete (the next one cannot start before this thread publishes P).  The last
                 // step takes the wait in any case: a parity wait can only tell the current phase from
                 // the one before it, and the final wait below must not find the barrier two behind.
                 // (pvDone completes one phase per tile, so its parity follows the running count.)
                 if (j > 0 && (rescale || j + 1u == myTiles)) {
-                    if (!pfWait<kCall>(&pvDone[x], (tt - 1u) & 1u, p.err, kDevErrMmaWait)) {
+                    if (!pvWait(tt - 1u)) {
                         ok = false;
                         break;
                     }
@@ -737,14 +751,6 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     tmemStWait();
                 }
                 m = mNew;
-                if (kAhead) {
-                    // the buffer's last probabilities, those of tile t - 2, have been multiplied (long ago as a rule)
-                    if (tt >= 2u && !pfWait<kCall>(&pvBuf[2u * x + b], ((tt - 2u) >> 1) & 1u, p.err, kDevErrMmaWait)) {
-                        ok = false;
-                        break;
-                    }
-                    tcFenceAfter();
-                }
                 // probabilities as fp16 pairs: the A operand of the PV product
                 // (every score of the row is already in registers)
                 // Pairs of elements with packed f32x2 arithmetic (scale-and-shift, row sum).  Evaluating
@@ -785,7 +791,7 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 if (row == 0) PF_STAMP(x, j, 2);
                 if (row == 0 && j + 1u == myTiles) PF_BLK(3u + x);
             }
-            ok = ok && (myTiles == 0 || pfWait<kCall>(&pvDone[x], (t + myTiles - 1u) & 1u, p.err, kDevErrMmaWait));
+            ok = ok && (myTiles == 0 || pvWait(t + myTiles - 1u));
             if (!ok) break;
             // Split items: each half leaves (m, l) of its rows for the other one and stores half of the dims, out of both
             // accumulators (they lie in the same TMEM lanes).
