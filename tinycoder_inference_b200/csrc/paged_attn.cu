@@ -53,20 +53,6 @@ struct PaL {
     static_assert(kBlocks * (kTotal + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
-__device__ __forceinline__ uint4 ldShared4(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint32_t sub1152(uint32_t x) {
-    const __half2 b = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-    __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&x), b);
-    return *reinterpret_cast<uint32_t *>(&h);
-}
-// bytes 0, 1 (2, 3) of w, each xor-ed with 0x80, as fp16 pairs
-__device__ __forceinline__ uint32_t bytesLo(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4140)); }
-__device__ __forceinline__ uint32_t bytesHi(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4342)); }
-
 __device__ __forceinline__ void pagedStore(const PagedAttnParams &p, uint32_t hd, uint32_t token0, uint32_t kvHead, uint32_t r, uint32_t dim, const float4 &x) {
     const uint32_t tok = token0 + r / p.group, head = kvHead * p.group + r % p.group;
     const size_t at = (static_cast<size_t>(tok) * p.nHeads + head) * hd + dim;
@@ -688,7 +674,7 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
     const uint32_t rows = maxTokens * p.group;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Sequences with many query rows go to the tensor cores' tiles, the others of the call to the rows kernel.
-    const bool tiles = half && !c->kvI8 && rows > kTilesFrom;
+    const bool tiles = half && rows > kTilesFrom;
     const bool rowsToo = !tiles || (c->starts != nullptr && c->batch > 1);
     uint32_t blocksA = 0;
     if (rowsToo) {

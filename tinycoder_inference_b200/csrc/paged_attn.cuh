@@ -185,6 +185,20 @@ struct PagedWalk {
         return true;
     }
 };
+__device__ __forceinline__ uint4 ldShared4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t sub1152(uint32_t x) {
+    const __half2 b = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&x), b);
+    return *reinterpret_cast<uint32_t *>(&h);
+}
+// bytes 0, 1 (2, 3) of w, each xor-ed with 0x80, as fp16 pairs
+__device__ __forceinline__ uint32_t bytesLo(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t bytesHi(uint32_t w) { return sub1152(__byte_perm(w, 0x64646464u, 0x4342)); }
+
 // The block's entry for the merge; one thread, whether the block has work or not.
 __device__ __forceinline__ void pagedLeaveJoin(const PagedAttnParams &p, const PagedWalk *w, uint32_t count) {
     PagedJoin j;
@@ -194,7 +208,7 @@ __device__ __forceinline__ void pagedLeaveJoin(const PagedAttnParams &p, const P
 }
 #endif
 
-// paged_tiles.cu: the sequences of minRows query rows per kv head and more, fp16 queries over an fp16 store, on tcgen05
+// paged_tiles.cu: the sequences of minRows query rows per kv head and more, fp16 queries, on tcgen05
 int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st);
 constexpr int kPagedSMs = 148;      // blocks that the workspace has room for, per block of an SM
 constexpr uint32_t kPagedTile = 128;  // query rows of a tile of the tiles kernel

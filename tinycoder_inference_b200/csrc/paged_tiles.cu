@@ -1,4 +1,4 @@
-// paged_tiles.cu -- attention of many query rows per kv head over an fp16 paged cache on tcgen05 (fp16 queries and results, f32
+// paged_tiles.cu -- attention of many query rows per kv head over a paged cache on tcgen05 (fp16 queries and results, f32
 // accumulation in TMEM): chunks of prompts and whole prompts.
 //
 // The block is prefill_f16.cu's: two 128-row query tiles A and B share a ring of 64-row K and V tiles, warps 0-3 / 4-7 hold the softmax of
@@ -9,6 +9,8 @@
 //   * K and V tiles are gathered page by page, a TMA copy per `box` rows, issued by the lanes of the producer warp side by side;
 //   * the work is the runs of paged_attn.cuh: a block's run of tiles may begin and end inside an item, whose partials the
 //     merge launch joins.  An item of one query tile gives its KV tiles to the two halves in turn (even / odd);
+//   * an int8 store's tiles go through three converter warps (13 - 15) to fp16 integers, exactly; a row's K scale comes to its scores and its V scale to
+//     its probabilities in f32.  The running maximum is then one of score + log2 of the largest V scale of the tile, so what P holds stays below 2^8;
 //   * rows past the sequence may hold anything: scores there are masked by selects, and the warp that issues P V writes zeros over V's.
 #include <cstring>
 
@@ -17,15 +19,20 @@
 
 namespace tc {
 
-constexpr int kPtThreads = 416;
+constexpr int kPtScales = 132;          // f32 of a scale slot: K's 64, V's 64, the power of two above V's; padding
+constexpr uint32_t kPtScaleSlots = 16;
 constexpr int kPtBN = int(kPaTile);
 constexpr float kPtLazyLog2 = 8.0f;  // O is rescaled when the row's maximum ran ahead by 2^8
+constexpr float kPtOff = 6.0f;       // probabilities are held as 2^6 p, at most 2^14: what fp16 has above them goes to the small ones
 
-template <int HD>
+template <int HD, bool I8>
 struct PtL {
+    static constexpr int kThreads = I8 ? 512 : 416;
     static constexpr int kHalves = HD / 64;
     static constexpr int kQTiles = HD > 128 ? 1 : 2;
-    static constexpr int NK = HD > 128 ? 2 : 6, NV = HD > 128 ? 2 : 4;
+    static constexpr int NK = HD > 128 ? 2 : I8 ? 3 : 6, NV = HD > 128 ? 2 : I8 ? 3 : 4;
+    static constexpr int NS = !I8 ? 0 : HD > 128 ? 3 : 6;      // int8: 64 x 128 byte panels on their way to the converters
+    static constexpr int kPanels = I8 ? HD / 128 : 1;          // ... of a tile
     static constexpr int kQHalf = int(kPagedTile) * 128;
     static constexpr int kKvHalf = kPtBN * 128;
     static constexpr int kQTile = kHalves * kQHalf;
@@ -33,10 +40,13 @@ struct PtL {
     static constexpr int kQ = 0;
     static constexpr int kK = kQTiles * kQTile;
     static constexpr int kV = kK + NK * kKvTile;
-    static constexpr int kExch = kV + NV * kKvTile;  // [half][row] (m, l) of items of one tile
+    static constexpr int kStaging = kV + NV * kKvTile;
+    static constexpr int kScale = kStaging + NS * kKvHalf;
+    static constexpr int kExch = kScale + (I8 ? int(kPtScaleSlots) * kPtScales * 4 : 0);  // [half][row] (m, l) of items of one tile
     static constexpr int kBars = kExch + (HD > 128 ? 0 : 2 * int(kPagedTile) * 8);
-    // qFull, kFull + kEmpty, vFull + vEmpty, sFull[2][2], pFull[2][2], pvBuf[2][2], qFree[2], exFull, exRead, sFree[2]
-    static constexpr int kNumBars = 1 + 2 * NK + 2 * NV + 4 + 4 + 4 + 2 + 2 + 2;
+    // qFull, kFull + kEmpty, vFull + vEmpty, sFull[2][2], pFull[2][2], pvDone[2], pvBuf[2][2], qFree[2], exFull, exRead, sFree[2],
+    // stFull + stEmpty
+    static constexpr int kNumBars = 1 + 2 * NK + 2 * NV + 4 + 4 + 2 + 4 + 2 + 2 + 2 + 2 * NS;
     static constexpr int kTmemSlot = kBars + kNumBars * 8;
     static constexpr int kTotal = kTmemSlot + 16;
     static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
@@ -71,21 +81,21 @@ __device__ __forceinline__ PtItem ptItem(const PagedAttnParams &p, const PagedWa
     return it;
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kPtThreads, 1)
+template <int HD, bool I8>
+__global__ void __launch_bounds__((PtL<HD, I8>::kThreads), 1)
 pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ PagedAttnParams p) {
-    using L = PtL<HD>;
+    using L = PtL<HD, I8>;
     constexpr int NC = kPtBN / 32;  // 32-column chunks of a score row
-    constexpr uint32_t NK = L::NK, NV = L::NV, BN = kPtBN;
+    constexpr uint32_t NK = L::NK, NV = L::NV, NS = L::NS, BN = kPtBN;
     constexpr bool kCall = HD < 256;
     constexpr bool kOne = L::kQTiles == 1;
     constexpr bool kAhead = kOne;   // one score buffer and two for probabilities (prefill_f16.cu)
     extern __shared__ __align__(1024) uint8_t smem[];  // (head_dim 128 has no room to round the address up)
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
     uint64_t *qFull = bars, *kFull = bars + 1, *kEmpty = kFull + NK, *vFull = kEmpty + NK, *vEmpty = vFull + NV, *sFull = vEmpty + NV /* [x][b] */,
-             *pFull = sFull + 4 /* [x][b] */, *pvBuf = pFull + 4 /* [x][b] */, *qFree = pvBuf + 4 /* [x] */,
-             *exFull = qFree + 2, *exRead = exFull + 1, *sFree = exRead + 1 /* [x] */;
+             *pFull = sFull + 4 /* [x][b] */, *pvDone = pFull + 4 /* [x] */, *pvBuf = pvDone + 2 /* [x][b] */, *qFree = pvBuf + 4 /* [x] */,
+             *exFull = qFree + 2, *exRead = exFull + 1, *sFree = exRead + 1 /* [x] */, *stFull = sFree + 2, *stEmpty = stFull + NS;
     uint32_t *tmemSlot = reinterpret_cast<uint32_t *>(smem + L::kTmemSlot);
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
     unsigned int *const err = p.c.err;
@@ -101,8 +111,9 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (threadIdx.x == 0) {
         mbarInit(qFull, 1);
         const uint32_t users = kOne ? 1u : 2u;  // a K (V) tile is released by the score (P.V) warps of both query tiles
-        for (uint32_t s = 0; s < NK; ++s) mbarInit(&kFull[s], 1), mbarInit(&kEmpty[s], users);
-        for (uint32_t s = 0; s < NV; ++s) mbarInit(&vFull[s], 1), mbarInit(&vEmpty[s], users);
+        for (uint32_t s = 0; s < NK; ++s) mbarInit(&kFull[s], L::kPanels), mbarInit(&kEmpty[s], users);
+        for (uint32_t s = 0; s < NV; ++s) mbarInit(&vFull[s], L::kPanels), mbarInit(&vEmpty[s], users);
+        for (uint32_t s = 0; s < NS; ++s) mbarInit(&stFull[s], 1), mbarInit(&stEmpty[s], 1);
         for (int i = 0; i < 4; ++i) {
             mbarInit(&sFull[i], 1);
             mbarInit(&pFull[i], 4);  // one arrival per warp
@@ -110,6 +121,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         for (int x = 0; x < 2; ++x) {
             mbarInit(&sFree[x], 4);
+            mbarInit(&pvDone[x], 1);
             mbarInit(&qFree[x], 1);
         }
         mbarInit(exFull, 2 * kPagedTile);
@@ -137,7 +149,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (!work) {
     } else if (warp == 8) {
         // ------------------------------- producer -------------------------------
-        uint32_t gk = 0, gv = 0, n = 0;
+        uint32_t gk = 0, gv = 0, gs = 0, n = 0;
         bool ok = true;
         const uint32_t boxes = BN / p.box, boxBytes = p.box * 128u;
         do {
@@ -155,6 +167,17 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         atomicOr(err, kDevErrRowBound);
                         page = 0;
                     }
+                }
+                if constexpr (I8) {  // panel by panel to the converters
+#pragma unroll
+                    for (int h = 0; h < L::kPanels; ++h, ++gs) {
+                        const uint32_t s = gs % (NS ? NS : 1u);
+                        if (gs >= NS && !pfWait<kCall>(&stEmpty[s], ((gs / (NS ? NS : 1u)) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
+                        if (lane == 0) mbarExpectTx(&stFull[s], have * boxBytes);
+                        __syncwarp();
+                        if (lane < have) tmaLoad4D(smem + L::kStaging + s * L::kKvHalf + lane * boxBytes, map, &stFull[s], 128 * h, w.kvHead, in, page);
+                    }
+                    return true;
                 }
                 const uint32_t s = g % N;
                 if (g >= N && !pfWait<kCall>(&empty[s], ((g / N) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
@@ -188,13 +211,85 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             for (uint32_t j = 0; ok && j < it.nTiles; ++j) ok = (j + 2u >= it.nTiles || requestK(j + 2u)) && requestV(j);
             ++n;
         } while (ok && w.next(p));
-        // the last release of every slot has to have arrived before the block leaves
-        for (uint32_t back = 1; ok && back <= NK && back <= gk; ++back) ok = pfWait<kCall>(&kEmpty[(gk - back) % NK], ((gk - back) / NK) & 1u, err, kDevErrEmptyWait);
-        for (uint32_t back = 1; ok && back <= NV && back <= gv; ++back) ok = pfWait<kCall>(&vEmpty[(gv - back) % NV], ((gv - back) / NV) & 1u, err, kDevErrEmptyWait);
-        if (!ok) {  // somebody gave up: the copies under way still land before the block leaves
-            for (uint32_t back = 1; back <= NK && back <= gk; ++back) pfWait<kCall>(&kFull[(gk - back) % NK], ((gk - back) / NK) & 1u, err, kDevErrFullWait);
-            for (uint32_t back = 1; back <= NV && back <= gv; ++back) pfWait<kCall>(&vFull[(gv - back) % NV], ((gv - back) / NV) & 1u, err, kDevErrFullWait);
+        // The last release of every slot has to have arrived before the block leaves; where somebody gave up, the copies under way
+        // still have to land.
+        auto drain = [&](uint64_t *bar, uint32_t count, uint32_t N, uint32_t bit) {
+            for (uint32_t back = 1; back <= N && back <= count; ++back)
+                if (!pfWait<kCall>(&bar[(count - back) % N], ((count - back) / N) & 1u, err, bit)) return false;
+            return true;
+        };
+        if constexpr (I8) {
+            if (!ok || !drain(stEmpty, gs, NS ? NS : 1u, kDevErrEmptyWait)) drain(stFull, gs, NS ? NS : 1u, kDevErrFullWait);
+        } else if (!ok || !drain(kEmpty, gk, NK, kDevErrEmptyWait) || !drain(vEmpty, gv, NV, kDevErrEmptyWait)) {
+            drain(kFull, gk, NK, kDevErrFullWait);
+            drain(vFull, gv, NV, kDevErrFullWait);
         }
+    } else if (I8 && warp >= 13) {
+        // ------------------------------ converters -----------------------------------
+        // Panels of 64 rows x 128 int8 in the order of the producer's requests, one warp each in turn, into two fp16 halves: rows of 64 dims
+        // under the same 128-byte swizzle.  K's converter of a tile brings its scales, and zero for V's past the sequence: what stands
+        // there is no number that a probability of 0 could be multiplied with.
+        const uint32_t me = warp - 13u;
+        uint32_t gs = 0, gk = 0, gv = 0;
+        bool ok = true;
+        do {
+            const PtItem it = ptItem<kOne>(p, w);
+            const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
+            auto convert = [&](uint32_t j, bool isK) {
+                uint32_t &g = isK ? gk : gv;
+                const uint32_t N = isK ? NK : NV, d = g % N;
+                uint64_t *full = isK ? kFull : vFull, *empty = isK ? kEmpty : vEmpty;
+#pragma unroll
+                for (int h = 0; h < L::kPanels; ++h, ++gs) {
+                    if (gs % 3u != me) continue;
+                    const uint32_t s = gs % (NS ? NS : 1u);
+                    if (g >= N && !pfWait<kCall>(&empty[d], ((g / N) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
+                    if (isK && h == 0) {
+                        // (a slot's last tile has been through the softmax: its score product was issued 16 - NK tiles ago)
+                        float *sc = reinterpret_cast<float *>(smem + L::kScale) + (g % kPtScaleSlots) * kPtScales;
+                        const uint32_t row0 = (it.t0 + j) * BN;
+                        uint32_t top = 0u;
+#pragma unroll
+                        for (uint32_t u = 0; u < 2; ++u) {
+                            const uint32_t key = lane + 32u * u, row = row0 + key;
+                            float a = 0.0f, b = 0.0f;
+                            if (row < w.s.len) {
+                                const uint32_t slot = row / p.c.pageRows;
+                                uint32_t page = static_cast<uint32_t>(__ldg(table + slot));
+                                if (page >= p.c.numPages) page = 0;
+                                const size_t at = (static_cast<size_t>(page) * p.c.pageRows + (row - slot * p.c.pageRows)) * p.c.nKV + w.kvHead;
+                                a = __ldg(p.ks + at), b = __ldg(p.vs + at);
+                            }
+                            sc[key] = a, sc[64u + key] = b;
+                            top = max(top, __float_as_uint(b) & 0x7fffffffu);
+                        }
+                        top = __reduce_max_sync(0xffffffffu, top);
+                        if (lane == 0) sc[128] = static_cast<float>(static_cast<int>(top >> 23) - 126);  // 2^that is above every scale
+                    }
+                    if (!pfWait<kCall>(&stFull[s], (gs / (NS ? NS : 1u)) & 1u, err, kDevErrFullWait)) return false;
+                    const uint32_t src = smemAddr(smem + L::kStaging + s * L::kKvHalf), dst = smemAddr(smem + (isK ? L::kK : L::kV) + d * L::kKvTile + 2 * h * L::kKvHalf);
+#pragma unroll 4
+                    for (uint32_t i = 0; i < 16u; ++i) {
+                        const uint32_t row = (lane & 7u) + 8u * (i >> 1), q = (lane >> 3) + 4u * (i & 1u), x = row & 7u;
+                        const uint4 v = ldShared4(src + row * 128u + ((q ^ x) << 4));
+                        const uint32_t a[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+                        const uint32_t out = dst + (q >> 2) * L::kKvHalf + row * 128u, c = 2u * (q & 3u);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + ((c ^ x) << 4)), "r"(bytesLo(a[0])), "r"(bytesHi(a[0])), "r"(bytesLo(a[1])), "r"(bytesHi(a[1])) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + (((c + 1u) ^ x) << 4)), "r"(bytesLo(a[2])), "r"(bytesHi(a[2])), "r"(bytesLo(a[3])), "r"(bytesHi(a[3])) : "memory");
+                    }
+                    fenceProxyAsync();  // the tensor cores read what this warp wrote; TMA writes next what it read
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbarArrive(&full[d]);
+                        mbarArrive(&stEmpty[s]);
+                    }
+                }
+                ++g;
+                return true;
+            };
+            ok = convert(0, true) && (it.nTiles < 2u || convert(1, true));
+            for (uint32_t j = 0; ok && j < it.nTiles; ++j) ok = (j + 2u >= it.nTiles || convert(j + 2u, true)) && convert(j, false);
+        } while (ok && w.next(p));
     } else if (warp >= 9) {
         // ------------------------------- MMA issuers -------------------------------
         // t counts the tiles of X over all items; tile t uses score buffer t % 2, which P(t - 2) has to have left (kAhead: the softmax
@@ -250,7 +345,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     ok = pfWait<kCall>(&vFull[s], (gg / NV) & 1u, err, kDevErrFullWait);
                     if (mine) {
                         const uint32_t row0 = (it.t0 + j) * BN;
-                        if (ok && row0 + BN > w.s.len) {
+                        if (!I8 && ok && row0 + BN > w.s.len) {
                             // rows past the sequence: zeros, whatever the pages (or an earlier tile) left there
                             const uint32_t keep = w.s.len > row0 ? w.s.len - row0 : 0u;
                             const uint32_t base = smemAddr(smem + L::kV + s * L::kKvTile);
@@ -271,6 +366,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             for (uint32_t ks = 0; ks < BN / 16; ++ks)  // 16 rows per step: 8 columns of fp16 P, 2 KB of V
                                 umaMmaTS(tO, tP + ks * 8u, descAdvance(dV, ks * 2048u), idPV, (tt > t || ks > 0) ? 1u : 0u);
                             umaCommit(&pvBuf[2u * x + (tt & 1u)]);
+                            if (!kAhead) umaCommit(&pvDone[x]);
                             umaCommit(&vEmpty[s]);
                         }
                         ++tt;
@@ -303,10 +399,16 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t laneBase = ((warp & 3u) * 32u) << 16;  // TMEM lane field
         const uint32_t tO = tmemBase + 128u * x;
         float2 *exch = reinterpret_cast<float2 *>(smem + L::kExch);
-        uint32_t t = 0, nSplit = 0;  // tiles of X, items of one tile so far
+        uint32_t t = 0, nSplit = 0, g = 0;  // tiles of X, items of one tile, KV tiles so far
         bool ok = true;
+        auto pvWait = [&](uint32_t tile) {  // the P.V product of that tile is complete
+            return kAhead ? pfWait<kCall>(&pvBuf[2u * x + (tile & 1u)], (tile >> 1) & 1u, err, kDevErrMmaWait)
+                          : pfWait<kCall>(&pvDone[x], tile & 1u, err, kDevErrMmaWait);
+        };
         do {
             const PtItem it = ptItem<kOne>(p, w);
+            const uint32_t g0 = g;
+            g += it.nTiles;
             const uint32_t myTiles = x == 0 ? it.nA : it.nB;
             const uint32_t myRows = it.split || x == 0u ? it.rowsA : it.rowsB;
             const uint32_t c0 = w.blockOf(w.item0), c1 = w.blockOf(w.item0 + w.tiles - 1u);
@@ -319,7 +421,9 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             float m = kNegBig, l = 0.0f;
             for (uint32_t j = 0; j < myTiles; ++j) {
                 const uint32_t tt = t + j, b = tt & 1u;
-                const int32_t kt = static_cast<int32_t>(it.t0 + (it.split ? 2u * j + x : j));  // KV tile
+                const uint32_t jj = it.split ? 2u * j + x : j;
+                const int32_t kt = static_cast<int32_t>(it.t0 + jj);  // KV tile
+                const float4 *sc = reinterpret_cast<const float4 *>(smem + L::kScale) + ((g0 + jj) % kPtScaleSlots) * (kPtScales / 4);
                 const uint32_t tS = tmemBase + 256u + 128u * x + (kAhead ? 0u : 64u * b), tP = kAhead ? tS + 64u + 32u * b : tS;
                 if (!pfWait<kCall>(&sFull[kAhead ? x : 2u * x + b], (kAhead ? tt : tt >> 1) & 1u, err, kDevErrMmaWait)) {
                     ok = false;
@@ -334,6 +438,17 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     tcFenceBefore();
                     __syncwarp();
                     if (lane == 0) mbarArrive(&sFree[x]);
+                }
+                if constexpr (I8) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 k = sc[8 * c + i / 4];
+                            const float2 a = __fmul2_rn(make_float2(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])), make_float2(k.x, k.y));
+                            const float2 b = __fmul2_rn(make_float2(__uint_as_float(r[c][i + 2]), __uint_as_float(r[c][i + 3])), make_float2(k.z, k.w));
+                            r[c][i] = __float_as_uint(a.x), r[c][i + 1] = __float_as_uint(a.y), r[c][i + 2] = __float_as_uint(b.x), r[c][i + 3] = __float_as_uint(b.y);
+                        }
                 }
                 if (kPtBN * kt + (kPtBN - 1) > pos0) {  // causal edge
                     const int32_t first = kPtBN * kt - pos;
@@ -351,7 +466,8 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             mxs[u] = max3(mxs[u], __uint_as_float(r[c][i + 2 * u]), __uint_as_float(r[c][i + 2 * u + 1]));
-                const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * p.scaleLog2;  // scale > 0: max commutes with it
+                const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * p.scaleLog2 +  // scale > 0: max commutes with it
+                                 (I8 ? reinterpret_cast<const float *>(sc)[128] : 0.0f);
                 const float mNew = mx > m + kPtLazyLog2 ? mx : m;
                 const bool rescale = j > 0 && __any_sync(0xffffffffu, mNew != m);
                 float alpha = 1.0f;
@@ -365,13 +481,16 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     tcFenceAfter();
                 }
-                if (rescale) {
-                    // O may only be touched between two of its P.V products
-                    if (!pfWait<kCall>(&pvBuf[2u * x + (b ^ 1u)], ((tt - 1u) >> 1) & 1u, err, kDevErrMmaWait)) {
+                // O may only be touched between two of its P.V products.  Without kAhead the wait goes by a barrier that completes a phase per tile;
+                // the last step takes it in any case, so that the wait behind the loop does not find the barrier two behind.
+                if (kAhead ? rescale : j > 0 && (rescale || j + 1u == myTiles)) {
+                    if (!pvWait(tt - 1u)) {
                         ok = false;
                         break;
                     }
                     tcFenceAfter();
+                }
+                if (rescale) {
                     alpha = fastExp2(m - mNew);
 #pragma unroll 1
                     for (uint32_t c = 0; c < HD / 32; ++c) {
@@ -385,7 +504,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     tmemStWait();
                 }
                 m = mNew;
-                const float2 scale2 = make_float2(p.scaleLog2, p.scaleLog2), negM2 = make_float2(-m, -m);
+                const float2 scale2 = make_float2(p.scaleLog2, p.scaleLog2), negM2 = make_float2(kPtOff - m, kPtOff - m);
                 float psum = 0.0f;
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
@@ -396,7 +515,12 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         const float2 x2 = __ffma2_rn(make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), scale2, negM2);
                         const float2 p2 = make_float2(fastExp2(x2.x), fastExp2(x2.y));
                         sum2 = __fadd2_rn(sum2, p2);
-                        h[i] = packHalf2(p2.x, p2.y);
+                        if constexpr (I8) {
+                            const float2 v = reinterpret_cast<const float2 *>(sc + 16)[16 * c + i], x = __fmul2_rn(p2, v);
+                            h[i] = packHalf2(x.x, x.y);
+                        } else {
+                            h[i] = packHalf2(p2.x, p2.y);
+                        }
                     }
                     psum += sum2.x + sum2.y;
                     tmemSt16(tP + laneBase + c * 16u, h);
@@ -407,10 +531,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbarArrive(&pFull[2u * x + b]);
             }
-            if (myTiles != 0u) {
-                const uint32_t tt = t + myTiles - 1u;
-                ok = ok && pfWait<kCall>(&pvBuf[2u * x + (tt & 1u)], (tt >> 1) & 1u, err, kDevErrMmaWait);
-            }
+            ok = ok && (myTiles == 0u || pvWait(t + myTiles - 1u));
             if (!ok) break;
             // Items of one query tile: each half leaves (m, l) of its rows for the other one and stores half of the dims, out of both
             // accumulators (they lie in the same TMEM lanes).
@@ -495,17 +616,17 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (warp == 0) tmemDealloc(tmemBase, 512);
 }
 
-template <int HD>
+template <int HD, bool I8>
 static int launchTiles(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const PagedAttnParams &p, cudaStream_t st) {
-    using L = PtL<HD>;
+    using L = PtL<HD, I8>;
     static bool attrDone[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !attrDone[dev]) {
-        TC_CUDA_OK(cudaFuncSetAttribute(pagedTilesKernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
+        TC_CUDA_OK(cudaFuncSetAttribute((pagedTilesKernel<HD, I8>), cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
         attrDone[dev] = true;
     }
-    return launchDependent(pagedTilesKernel<HD>, dim3(numSMs() < kPagedSMs ? numSMs() : kPagedSMs), kPtThreads, L::kTotal, st, 1, q, k, v, p);
+    return launchDependent(pagedTilesKernel<HD, I8>, dim3(numSMs() < kPagedSMs ? numSMs() : kPagedSMs), L::kThreads, L::kTotal, st, 1, q, k, v, p);
 }
 
 int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st) {
@@ -522,8 +643,9 @@ int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st) {
     key.rank = 3, key.elemBytes = 2, key.swizzle = 3;
     rc = getTensorMap(key, &q);
     if (rc != TC_OK) return rc;
-    if (c->hd == 64) return launchTiles<64>(q, k, v, p, st);
-    return c->hd == 128 ? launchTiles<128>(q, k, v, p, st) : launchTiles<256>(q, k, v, p, st);
+    if (c->kvI8) return c->hd == 128 ? launchTiles<128, true>(q, k, v, p, st) : launchTiles<256, true>(q, k, v, p, st);
+    if (c->hd == 64) return launchTiles<64, false>(q, k, v, p, st);
+    return c->hd == 128 ? launchTiles<128, false>(q, k, v, p, st) : launchTiles<256, false>(q, k, v, p, st);
 }
 
 }  // namespace tc
