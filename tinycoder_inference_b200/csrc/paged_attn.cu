@@ -199,18 +199,29 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         do {
             const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
             const uint32_t t1 = w.last();
-            for (uint32_t t = w.first(); t < t1; ++t, ++g) {
+            // where this lane's box of a tile lies: looked up a tile ahead
+            struct At {
+                uint32_t have, in;
+                int32_t page;
+            };
+            auto look = [&](uint32_t t) {
                 const uint32_t row0 = t * kPaTile;
-                const uint32_t n = w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u;
-                uint32_t page = 0, in = 0;
-                if (lane < n) {
+                At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
+                if (lane < at.have) {
                     const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
-                    in = row - slot * p.c.pageRows;
-                    page = static_cast<uint32_t>(__ldg(table + slot));
-                    if (page >= p.c.numPages) {  // no such page: reported, page 0 stands in
-                        atomicOr(p.c.err, kDevErrRowBound);
-                        page = 0;
-                    }
+                    at.in = row - slot * p.c.pageRows;
+                    at.page = __ldg(table + slot);
+                }
+                return at;
+            };
+            At next = look(w.first());
+            for (uint32_t t = w.first(); t < t1; ++t, ++g) {
+                const uint32_t n = next.have, in = next.in;
+                uint32_t page = static_cast<uint32_t>(next.page);
+                next = look(t + 1u);
+                if (lane < n && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
+                    atomicOr(p.c.err, kDevErrRowBound);
+                    page = 0;
                 }
                 const uint32_t st = g % NST;
                 if (g >= NST) ok = pfWait<true>(&empty[st], ((g / NST) - 1u) & 1u, p.c.err, kDevErrEmptyWait);

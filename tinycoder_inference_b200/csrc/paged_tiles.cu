@@ -25,6 +25,49 @@ constexpr int kPtBN = int(kPaTile);
 constexpr float kPtLazyLog2 = 8.0f;  // O is rescaled when the row's maximum ran ahead by 2^8
 constexpr float kPtOff = 6.0f;       // probabilities are held as 2^6 p, at most 2^14: what fp16 has above them goes to the small ones
 
+// What a block has of an item, as its producer hands it to the other warps (in shared memory: the walk's state would cost the softmax
+// threads registers that they spill for).  Tiles j = 0 .. nTiles - 1 are cache rows 64 (t0 + j) ..; query tile X takes tile j if
+// mine(X, j).  nTiles 0: the run is done.
+struct PtItem {
+    uint32_t nTiles, t0, nA, nB;
+    uint32_t m0, rowsA, rowsB;                // first row; rows of A and B
+    uint32_t split, whole;                    // one query tile for both halves; the item is the block's alone
+    uint32_t seq, kvHead, token0, len, part;  // part: the partial's slot
+    int32_t before;
+    uint32_t pad;
+    __device__ __forceinline__ bool mine(uint32_t x, uint32_t j) const { return split ? (j & 1u) == x : j < (x == 0u ? nA : nB); }
+};
+constexpr uint32_t kPtItems = 8;  // (the producer is two items ahead of the score products, which are at most two tiles ahead of the softmax)
+template <bool ONE>
+__device__ __forceinline__ PtItem ptItem(const PagedAttnParams &p, const PagedWalk &w, uint32_t &joins) {
+    PtItem it;
+    const uint32_t tile = p.tileTokens * p.group;
+    it.m0 = w.item * w.mr;
+    const uint32_t rows = min(w.mr, w.s.rows - it.m0);
+    it.rowsA = min(rows, tile), it.rowsB = rows - it.rowsA;
+    it.t0 = w.first();
+    const uint32_t t1 = w.last();
+    it.nTiles = t1 - it.t0;
+    it.whole = it.t0 == 0u && t1 == w.tiles;
+    it.split = !ONE && it.rowsB == 0u;
+    if (it.split) {
+        it.nB = it.nTiles / 2u, it.nA = it.nTiles - it.nB;
+    } else {
+        // A's rows end before B's
+        const uint32_t tilesA = it.rowsB == 0u ? w.tiles : min(w.tiles, max(1u, (w.s.sees(it.m0 + it.rowsA, p.group) + kPaTile - 1u) / kPaTile));
+        it.nA = min(t1, tilesA) > it.t0 ? min(t1, tilesA) - it.t0 : 0u;
+        it.nB = it.rowsB != 0u ? it.nTiles : 0u;
+    }
+    it.seq = w.seq, it.kvHead = w.kvHead, it.token0 = w.s.token0, it.len = w.s.len, it.before = w.s.before;
+    it.part = 0, joins = 0, it.pad = 0;
+    if (!it.whole) {
+        const uint32_t c0 = w.blockOf(w.item0), c1 = w.blockOf(w.item0 + w.tiles - 1u);
+        it.part = blockIdx.x == c0 ? 1u : 0u;
+        if (blockIdx.x == c0) joins = c1 - c0 + 1u;
+    }
+    return it;
+}
+
 template <int HD, bool I8>
 struct PtL {
     static constexpr int kThreads = I8 ? 512 : 416;
@@ -45,41 +88,13 @@ struct PtL {
     static constexpr int kExch = kScale + (I8 ? int(kPtScaleSlots) * kPtScales * 4 : 0);  // [half][row] (m, l) of items of one tile
     static constexpr int kBars = kExch + (HD > 128 ? 0 : 2 * int(kPagedTile) * 8);
     // qFull, kFull + kEmpty, vFull + vEmpty, sFull[2][2], pFull[2][2], pvDone[2], pvBuf[2][2], qFree[2], exFull, exRead, sFree[2],
-    // stFull + stEmpty
-    static constexpr int kNumBars = 1 + 2 * NK + 2 * NV + 4 + 4 + 2 + 4 + 2 + 2 + 2 + 2 * NS;
+    // stFull + stEmpty, itemFull
+    static constexpr int kNumBars = 1 + 2 * NK + 2 * NV + 4 + 4 + 2 + 4 + 2 + 2 + 2 + 2 * NS + int(kPtItems);
     static constexpr int kTmemSlot = kBars + kNumBars * 8;
-    static constexpr int kTotal = kTmemSlot + 16;
+    static constexpr int kItems = (kTmemSlot + 16 + 15) / 16 * 16;
+    static constexpr int kTotal = kItems + int(kPtItems) * int(sizeof(PtItem));
     static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
 };
-
-// What a block has of an item: tiles j = 0 .. nTiles - 1 are cache rows 64 (t0 + j) ..; query tile X takes tile j if mine(X, j).
-struct PtItem {
-    uint32_t m0, rowsA, rowsB, t0, nTiles, nA, nB;
-    bool split, whole;
-    __device__ __forceinline__ bool mine(uint32_t x, uint32_t j) const { return split ? (j & 1u) == x : j < (x == 0u ? nA : nB); }
-};
-template <bool ONE>
-__device__ __forceinline__ PtItem ptItem(const PagedAttnParams &p, const PagedWalk &w) {
-    PtItem it;
-    const uint32_t tile = p.tileTokens * p.group;
-    it.m0 = w.item * w.mr;
-    const uint32_t rows = min(w.mr, w.s.rows - it.m0);
-    it.rowsA = min(rows, tile), it.rowsB = rows - it.rowsA;
-    it.t0 = w.first();
-    const uint32_t t1 = w.last();
-    it.nTiles = t1 - it.t0;
-    it.whole = it.t0 == 0u && t1 == w.tiles;
-    it.split = !ONE && it.rowsB == 0u;
-    if (it.split) {
-        it.nB = it.nTiles / 2u, it.nA = it.nTiles - it.nB;
-    } else {
-        // A's rows end before B's
-        const uint32_t tilesA = it.rowsB == 0u ? w.tiles : min(w.tiles, max(1u, (w.s.sees(it.m0 + it.rowsA, p.group) + kPaTile - 1u) / kPaTile));
-        it.nA = min(t1, tilesA) > it.t0 ? min(t1, tilesA) - it.t0 : 0u;
-        it.nB = it.rowsB != 0u ? it.nTiles : 0u;
-    }
-    return it;
-}
 
 template <int HD, bool I8>
 __global__ void __launch_bounds__((PtL<HD, I8>::kThreads), 1)
@@ -95,7 +110,8 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
     uint64_t *qFull = bars, *kFull = bars + 1, *kEmpty = kFull + NK, *vFull = kEmpty + NK, *vEmpty = vFull + NV, *sFull = vEmpty + NV /* [x][b] */,
              *pFull = sFull + 4 /* [x][b] */, *pvDone = pFull + 4 /* [x] */, *pvBuf = pvDone + 2 /* [x][b] */, *qFree = pvBuf + 4 /* [x] */,
-             *exFull = qFree + 2, *exRead = exFull + 1, *sFree = exRead + 1 /* [x] */, *stFull = sFree + 2, *stEmpty = stFull + NS;
+             *exFull = qFree + 2, *exRead = exFull + 1, *sFree = exRead + 1 /* [x] */, *stFull = sFree + 2, *stEmpty = stFull + NS, *itemFull = stEmpty + NS;
+    PtItem *items = reinterpret_cast<PtItem *>(smem + L::kItems);
     uint32_t *tmemSlot = reinterpret_cast<uint32_t *>(smem + L::kTmemSlot);
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
     unsigned int *const err = p.c.err;
@@ -124,6 +140,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             mbarInit(&pvDone[x], 1);
             mbarInit(&qFree[x], 1);
         }
+        for (uint32_t i = 0; i < kPtItems; ++i) mbarInit(&itemFull[i], 1);
         mbarInit(exFull, 2 * kPagedTile);
         mbarInit(exRead, 2 * kPagedTile);
         fenceBarrierInit();
@@ -142,31 +159,52 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     gridDepWait();
     gridDepLaunch();
     const uint32_t tileRows = p.tileTokens * p.group;
-    if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
-    PagedWalk w;
-    const bool work = w.begin(p, tileRows * L::kQTiles);
+    // The n-th item of the block, once the producer has put it down; false: there is none any more.
+    auto takeItem = [&](uint32_t n, const PtItem *&it) {
+        it = &items[n % kPtItems];
+        return pfWait<kCall>(&itemFull[n % kPtItems], (n / kPtItems) & 1u, err, kDevErrFullWait) && it->nTiles != 0u;
+    };
 
-    if (!work) {
-    } else if (warp == 8) {
+    if (warp == 8) {
         // ------------------------------- producer -------------------------------
         uint32_t gk = 0, gv = 0, gs = 0, n = 0;
-        bool ok = true;
         const uint32_t boxes = BN / p.box, boxBytes = p.box * 128u;
-        do {
-            const PtItem it = ptItem<kOne>(p, w);
+        if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
+        PagedWalk w;
+        const bool some = w.begin(p, tileRows * L::kQTiles);
+        bool ok = true;
+        if (some) do {
+            uint32_t joins;
+            const PtItem it = ptItem<kOne>(p, w, joins);
+            if (lane == 0) {
+                items[n % kPtItems] = it;
+                mbarArrive(&itemFull[n % kPtItems]);
+                if (joins != 0u) pagedLeaveJoin(p, &w, joins);
+            }
+            ++n;
             const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
-            auto request = [&](uint32_t j, const CUtensorMap *map, uint32_t base, uint64_t *full, uint64_t *empty, uint32_t &g, uint32_t N) {
+            // Where this lane's box of tile j lies.  Looked up a tile ahead of its first use: a request that waits for its table entry
+            // falls behind the products.
+            struct At {
+                uint32_t have, in;
+                int32_t page;
+            };
+            auto look = [&](uint32_t j) {
                 const uint32_t row0 = (it.t0 + j) * BN;
-                const uint32_t have = w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u;
-                uint32_t page = 0, in = 0;
-                if (lane < have) {
+                At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
+                if (lane < at.have) {
                     const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
-                    in = row - slot * p.c.pageRows;
-                    page = static_cast<uint32_t>(__ldg(table + slot));
-                    if (page >= p.c.numPages) {  // no such page: reported, page 0 stands in
-                        atomicOr(err, kDevErrRowBound);
-                        page = 0;
-                    }
+                    at.in = row - slot * p.c.pageRows;
+                    at.page = __ldg(table + slot);
+                }
+                return at;
+            };
+            auto request = [&](const At &at, const CUtensorMap *map, uint32_t base, uint64_t *full, uint64_t *empty, uint32_t &g, uint32_t N) {
+                const uint32_t have = at.have, in = at.in;
+                uint32_t page = static_cast<uint32_t>(at.page);
+                if (lane < have && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
+                    atomicOr(err, kDevErrRowBound);
+                    page = 0;
                 }
                 if constexpr (I8) {  // panel by panel to the converters
 #pragma unroll
@@ -191,11 +229,12 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 ++g;
                 return true;
             };
-            auto requestK = [&](uint32_t j) { return request(j, &tmK, L::kK, kFull, kEmpty, gk, NK); };
-            auto requestV = [&](uint32_t j) { return request(j, &tmV, L::kV, vFull, vEmpty, gv, NV); };
+            auto requestK = [&](const At &at) { return request(at, &tmK, L::kK, kFull, kEmpty, gk, NK); };
+            auto requestV = [&](const At &at) { return request(at, &tmV, L::kV, vFull, vEmpty, gv, NV); };
+            At a0 = look(0), a1 = look(1), a2 = look(2);  // tiles j, j + 1, j + 2 (rows past the run's last tile are only looked up)
             // the query tiles are free once the last score products of the previous item are complete
-            if (n > 0)
-                ok = pfWait<kCall>(&qFree[0], (n - 1u) & 1u, err, kDevErrEmptyWait) && (kOne || pfWait<kCall>(&qFree[1], (n - 1u) & 1u, err, kDevErrEmptyWait));
+            if (n > 1u)
+                ok = pfWait<kCall>(&qFree[0], n & 1u, err, kDevErrEmptyWait) && (kOne || pfWait<kCall>(&qFree[1], n & 1u, err, kDevErrEmptyWait));
             if (!ok) break;
             if (lane == 0) {
                 const uint32_t qTiles = it.rowsB != 0u ? 2u : 1u;
@@ -207,10 +246,17 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                                   w.s.token0 + it.m0 / p.group + x * p.tileTokens);
             }
             __syncwarp();
-            ok = requestK(0) && (it.nTiles < 2u || requestK(1));
-            for (uint32_t j = 0; ok && j < it.nTiles; ++j) ok = (j + 2u >= it.nTiles || requestK(j + 2u)) && requestV(j);
-            ++n;
+            ok = requestK(a0) && (it.nTiles < 2u || requestK(a1));
+            for (uint32_t j = 0; ok && j < it.nTiles; ++j) {
+                const At a3 = look(j + 3u);
+                ok = (j + 2u >= it.nTiles || requestK(a2)) && requestV(a0);
+                a0 = a1, a1 = a2, a2 = a3;
+            }
         } while (ok && w.next(p));
+        if (lane == 0) {
+            items[n % kPtItems].nTiles = 0u;
+            mbarArrive(&itemFull[n % kPtItems]);
+        }
         // The last release of every slot has to have arrived before the block leaves; where somebody gave up, the copies under way
         // still have to land.
         auto drain = [&](uint64_t *bar, uint32_t count, uint32_t N, uint32_t bit) {
@@ -232,9 +278,10 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t me = warp - 13u;
         uint32_t gs = 0, gk = 0, gv = 0;
         bool ok = true;
-        do {
-            const PtItem it = ptItem<kOne>(p, w);
-            const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
+        const PtItem *at;
+        for (uint32_t n = 0; ok && takeItem(n, at); ++n) {
+            const PtItem it = *at;
+            const int32_t *table = p.c.pages + static_cast<size_t>(it.seq) * p.c.pagesPerSeq;
             auto convert = [&](uint32_t j, bool isK) {
                 uint32_t &g = isK ? gk : gv;
                 const uint32_t N = isK ? NK : NV, d = g % N;
@@ -253,11 +300,11 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (uint32_t u = 0; u < 2; ++u) {
                             const uint32_t key = lane + 32u * u, row = row0 + key;
                             float a = 0.0f, b = 0.0f;
-                            if (row < w.s.len) {
+                            if (row < it.len) {
                                 const uint32_t slot = row / p.c.pageRows;
                                 uint32_t page = static_cast<uint32_t>(__ldg(table + slot));
                                 if (page >= p.c.numPages) page = 0;
-                                const size_t at = (static_cast<size_t>(page) * p.c.pageRows + (row - slot * p.c.pageRows)) * p.c.nKV + w.kvHead;
+                                const size_t at = (static_cast<size_t>(page) * p.c.pageRows + (row - slot * p.c.pageRows)) * p.c.nKV + it.kvHead;
                                 a = __ldg(p.ks + at), b = __ldg(p.vs + at);
                             }
                             sc[key] = a, sc[64u + key] = b;
@@ -289,7 +336,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             };
             ok = convert(0, true) && (it.nTiles < 2u || convert(1, true));
             for (uint32_t j = 0; ok && j < it.nTiles; ++j) ok = (j + 2u >= it.nTiles || convert(j + 2u, true)) && convert(j, false);
-        } while (ok && w.next(p));
+        }
     } else if (warp >= 9) {
         // ------------------------------- MMA issuers -------------------------------
         // t counts the tiles of X over all items; tile t uses score buffer t % 2, which P(t - 2) has to have left (kAhead: the softmax
@@ -303,10 +350,11 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint64_t dK0 = umaSmemDesc(smemAddr(smem + L::kK), 16, 1024);
         const uint64_t dV0 = umaSmemDesc(smemAddr(smem + L::kV), L::kKvHalf, 1024);
         const uint32_t tO = tmemBase + 128u * x, tS0 = tmemBase + 256u + 128u * x;
-        uint32_t g = 0, t = 0, n = 0;
-        bool ok = true;
-        if (!(kOne && x == 1u)) do {
-            const PtItem it = ptItem<kOne>(p, w);
+        uint32_t g = 0, t = 0;
+        bool ok = !(kOne && x == 1u);
+        const PtItem *at;
+        for (uint32_t n = 0; ok && takeItem(n, at); ++n) {
+            const PtItem it = *at;
             const uint32_t myTiles = x == 0 ? it.nA : it.nB;
             const uint64_t dQ = descAdvance(dQ0, it.split ? 0u : x * L::kQTile);
             uint32_t tt = t;
@@ -345,9 +393,9 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     ok = pfWait<kCall>(&vFull[s], (gg / NV) & 1u, err, kDevErrFullWait);
                     if (mine) {
                         const uint32_t row0 = (it.t0 + j) * BN;
-                        if (!I8 && ok && row0 + BN > w.s.len) {
+                        if (!I8 && ok && row0 + BN > it.len) {
                             // rows past the sequence: zeros, whatever the pages (or an earlier tile) left there
-                            const uint32_t keep = w.s.len > row0 ? w.s.len - row0 : 0u;
+                            const uint32_t keep = it.len > row0 ? it.len - row0 : 0u;
                             const uint32_t base = smemAddr(smem + L::kV + s * L::kKvTile);
                             for (uint32_t i = lane; i < (BN - keep) * 8u * L::kHalves; i += 32u) {
                                 const uint32_t chunk = i & 7u, row = keep + (i >> 3) % (BN - keep), h = (i >> 3) / (BN - keep);
@@ -385,8 +433,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             t += myTiles;
             g += it.nTiles;
-            ++n;
-        } while (ok && w.next(p));
+        }
         if (pvRole && ok) {
             // the last two buffer commits have to land before the block leaves
             for (uint32_t tt = t >= 2u ? t - 2u : 0u; tt < t; ++tt)
@@ -405,24 +452,25 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             return kAhead ? pfWait<kCall>(&pvBuf[2u * x + (tile & 1u)], (tile >> 1) & 1u, err, kDevErrMmaWait)
                           : pfWait<kCall>(&pvDone[x], tile & 1u, err, kDevErrMmaWait);
         };
-        do {
-            const PtItem it = ptItem<kOne>(p, w);
+        const PtItem *at;
+        for (uint32_t n = 0; ok && takeItem(n, at); ++n) {
+            const PtItem &it = *at;
             const uint32_t g0 = g;
             g += it.nTiles;
             const uint32_t myTiles = x == 0 ? it.nA : it.nB;
-            const uint32_t myRows = it.split || x == 0u ? it.rowsA : it.rowsB;
-            const uint32_t c0 = w.blockOf(w.item0), c1 = w.blockOf(w.item0 + w.tiles - 1u);
-            if (threadIdx.x == 0 && !it.whole && blockIdx.x == c0) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
-            if (myRows == 0u) continue;  // (no query tile B)
-            const uint32_t tileRow0 = it.split ? 0u : x * tileRows;          // the tile's first row inside the item
-            const uint32_t rr = it.m0 + tileRow0 + row, tok = rr / p.group;  // row and token of the sequence
-            const int32_t pos = w.s.before + static_cast<int32_t>(tok);      // the last cache row that the query row sees
-            const int32_t pos0 = w.s.before + static_cast<int32_t>((it.m0 + tileRow0) / p.group);  // ... that the tile's first row does
+            const bool split = it.split != 0u;
+            const uint32_t tileRow0 = split ? 0u : x * tileRows, t0 = it.t0;  // the tile's first row inside the item
+            int32_t pos, pos0;                                                // the last cache row that the query row (the tile's first row) sees
+            {
+                const uint32_t first = it.m0 + tileRow0;
+                pos = it.before + static_cast<int32_t>((first + row) / p.group);
+                pos0 = it.before + static_cast<int32_t>(first / p.group);
+            }
             float m = kNegBig, l = 0.0f;
             for (uint32_t j = 0; j < myTiles; ++j) {
                 const uint32_t tt = t + j, b = tt & 1u;
-                const uint32_t jj = it.split ? 2u * j + x : j;
-                const int32_t kt = static_cast<int32_t>(it.t0 + jj);  // KV tile
+                const uint32_t jj = split ? 2u * j + x : j;
+                const int32_t kt = static_cast<int32_t>(t0 + jj);  // KV tile
                 const float4 *sc = reinterpret_cast<const float4 *>(smem + L::kScale) + ((g0 + jj) % kPtScaleSlots) * (kPtScales / 4);
                 const uint32_t tS = tmemBase + 256u + 128u * x + (kAhead ? 0u : 64u * b), tP = kAhead ? tS + 64u + 32u * b : tS;
                 if (!pfWait<kCall>(&sFull[kAhead ? x : 2u * x + b], (kAhead ? tt : tt >> 1) & 1u, err, kDevErrMmaWait)) {
@@ -536,7 +584,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             // Items of one query tile: each half leaves (m, l) of its rows for the other one and stores half of the dims, out of both
             // accumulators (they lie in the same TMEM lanes).
             float M = m, lAll = l, wMine = 1.0f, wOther = 0.0f;
-            if (it.split) {
+            if (split) {
                 exch[x * kPagedTile + row] = make_float2(m, l);
                 tcFenceBefore();
                 mbarArrive(exFull);
@@ -549,15 +597,19 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             } else {
                 tcFenceAfter();
             }
-            const bool other = it.split && (x == 0u ? it.nB : it.nA) != 0u, own = myTiles != 0u;  // accumulators that were written
-            const float inv = it.whole ? (lAll == 0.0f ? 0.0f : 1.0f / lAll) : 1.0f;
+            const bool other = split && (x == 0u ? it.nB : it.nA) != 0u, own = myTiles != 0u;  // accumulators that were written
+            const bool whole = it.whole != 0u;
+            const uint32_t myRows = split || x == 0u ? it.rowsA : it.rowsB;
+            const float inv = whole ? (lAll == 0.0f ? 0.0f : 1.0f / lAll) : 1.0f;
             wMine *= inv, wOther *= inv;
             constexpr uint32_t kChunks = HD / 32;
-            const uint32_t k0 = it.split ? x * (kChunks / 2) : 0u, k1 = it.split ? k0 + kChunks / 2 : kChunks;
+            const uint32_t k0 = split ? x * (kChunks / 2) : 0u, k1 = split ? k0 + kChunks / 2 : kChunks;
             const uint32_t local = tileRow0 + row;  // row of the item
-            float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + (blockIdx.x == c0 ? 1u : 0u)) * pagedSlot(w.mr, HD);
-            if (!it.whole && row < myRows && (!it.split || x == 0u)) part[w.mr * HD + local] = M, part[w.mr * HD + w.mr + local] = lAll;
-            __half *orow = static_cast<__half *>(p.out) + (static_cast<size_t>(w.s.token0 + tok) * p.nHeads + w.kvHead * p.group + (rr - tok * p.group)) * HD;
+            const uint32_t mr = tileRows * L::kQTiles;
+            float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + it.part) * pagedSlot(mr, HD);
+            if (!whole && row < myRows && (!split || x == 0u)) part[mr * HD + local] = M, part[mr * HD + mr + local] = lAll;
+            const uint32_t rr = it.m0 + local, tok = rr / p.group;
+            __half *orow = static_cast<__half *>(p.out) + (static_cast<size_t>(it.token0 + tok) * p.nHeads + it.kvHead * p.group + (rr - tok * p.group)) * HD;
 #pragma unroll 1
             for (uint32_t c = k0; c < k1; ++c) {
                 uint32_t o[32];
@@ -577,7 +629,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), wOther, __uint_as_float(o[i])));
                 }
-                if (row < myRows && !it.whole) {
+                if (row < myRows && !whole) {
                     // 32 bytes per store: a thread owns its row
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -600,7 +652,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                 }
             }
-            if (it.split) {
+            if (split) {
                 // the next item's first P.V product may overwrite an accumulator once both halves have read it
                 tcFenceBefore();
                 mbarArrive(exRead);
@@ -610,7 +662,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 tcFenceBefore();
             }
             t += myTiles;
-        } while (ok && w.next(p));
+        }
     }
     __syncthreads();
     if (warp == 0) tmemDealloc(tmemBase, 512);
