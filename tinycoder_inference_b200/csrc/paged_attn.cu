@@ -25,6 +25,10 @@
 
 namespace tc {
 
+#ifndef PA_OVER
+#define PA_OVER 0
+#endif
+constexpr uint32_t kPaOver = PA_OVER;
 constexpr int kPaThreads = 160;       // four consumer warps, one producer warp
 // The workspace: two partials per block of the two kernels' widest grids, then what the merge finds per block.
 constexpr size_t kRowsParts = size_t(2) * kPagedSMs * 2 * pagedSlot(64, 128);       // f32
@@ -189,7 +193,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     gridDepLaunch();
     PagedWalk w;
     if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
-    if (!w.begin(p, MR)) return;
+    if (!w.begin(p, MR, kPaOver)) return;
     bool ok = true;
     uint32_t g = 0;  // tiles so far
 
@@ -537,7 +541,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             }
         }
         const bool whole = t0 == 0u && t1 == w.tiles;
-        const uint32_t c0 = w.blockOf(w.item0), c1 = w.blockOf(w.item0 + w.tiles - 1u);
+        const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
         float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + (blockIdx.x == c0 ? 1u : 0u)) * pagedSlot(MR, HD);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -701,7 +705,7 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
         const int rb = pagedAttnTiles(c, b, st);
         if (rb != TC_OK) return rb;
     }
-    const dim3 grid(blocksA + (tiles ? std::min(numSMs(), kPagedSMs) : 0), 8);
+    const dim3 grid(blocksA + (tiles ? std::min(numSMs(), kPagedSMs) : 0), tiles ? 32 : 8);
     auto merge = c->hd == 64 ? pagedMergeKernel<64> : c->hd == 128 ? pagedMergeKernel<128> : pagedMergeKernel<256>;
     return launchDependent(merge, grid, 256, 0, st, 1, p, static_cast<const float *>(partsB), static_cast<const PagedJoin *>(joinsB), blocksA);
 }

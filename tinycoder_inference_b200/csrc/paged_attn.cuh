@@ -3,7 +3,7 @@
 // An item is up to MR consecutive query rows of one kv head of one sequence; query row r of a sequence's kv head is q head
 // r % group of its token r / group, so the heads that share K and V sit side by side and one pass over the rows serves them.  A
 // unit is one tile of kPaTile cache rows of an item.  The units of all items in a row -- sequence, kv head, rows -- are cut into
-// equal runs, one per block: ragged lengths, single tokens and prompts fill the SMs alike.  An item that lies in several runs
+// equal runs, one per block (an item counts some units more than its tiles, for what it costs beside them): ragged lengths, single tokens and prompts fill the SMs alike.  An item that lies in several runs
 // is put together by a second launch from partials in the workspace.
 #pragma once
 
@@ -102,7 +102,7 @@ __device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, uint32_t 
 
 // A walk over a block's run of units, item by item; every warp makes its own, in step.
 struct PagedWalk {
-    uint32_t mr;              // query rows of an item
+    uint32_t mr, over;        // query rows of an item; units ahead of its tiles that stand for what an item costs beside them
     uint64_t total, at, end;  // units of the launch; the block's next and last
     uint32_t blocks;          // blocks with work
     uint32_t seq, kvHead, item;
@@ -113,13 +113,16 @@ struct PagedWalk {
     __device__ __forceinline__ uint64_t firstOf(uint32_t block) const { return static_cast<uint64_t>(block) * total / blocks; }
     __device__ __forceinline__ uint32_t blockOf(uint64_t unit) const { return static_cast<uint32_t>(((unit + 1u) * blocks - 1u) / total); }
 
+    __device__ __forceinline__ uint64_t unitsAll(const PagedSeq &q, uint32_t group) const { return q.tilesAll(mr, group) + static_cast<uint64_t>(over) * q.items(mr); }
+    __device__ __forceinline__ uint64_t unitsBefore(uint32_t m, uint32_t group) const { return s.tilesBefore(mr, m, group) + static_cast<uint64_t>(over) * m; }
+
     // All lanes of the warp.  False: nothing to do.
-    __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows) {
-        mr = itemRows;
+    __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
+        mr = itemRows, over = overhead;
         const uint32_t lane = threadIdx.x & 31u;
         uint64_t sum = 0;
         for (uint32_t b0 = 0; b0 < p.c.batch; b0 += 32u)
-            if (b0 + lane < p.c.batch) sum += pagedSeq(p, b0 + lane).tilesAll(mr, p.group) * p.c.nKV;
+            if (b0 + lane < p.c.batch) sum += unitsAll(pagedSeq(p, b0 + lane), p.group) * p.c.nKV;
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum;
@@ -131,7 +134,7 @@ struct PagedWalk {
         uint64_t base = 0;
         for (uint32_t b0 = 0;; b0 += 32u) {
             uint64_t mine = 0;
-            if (b0 + lane < p.c.batch) mine = pagedSeq(p, b0 + lane).tilesAll(mr, p.group) * p.c.nKV;
+            if (b0 + lane < p.c.batch) mine = unitsAll(pagedSeq(p, b0 + lane), p.group) * p.c.nKV;
             uint64_t upTo = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -149,28 +152,30 @@ struct PagedWalk {
             if (b0 + 32u >= p.c.batch) return false;  // (not reached: `at` lies below the sum)
         }
         s = pagedSeq(p, seq);
-        const uint64_t per = s.tilesAll(mr, p.group);
+        const uint64_t per = unitsAll(s, p.group);
         kvHead = static_cast<uint32_t>((at - base) / per);
         const uint64_t in = at - base - kvHead * per;
         uint32_t lo = 0, hi = s.items(mr) - 1u;  // the last item whose first tile is not behind `in`
         while (lo < hi) {
             const uint32_t mid = (lo + hi + 1u) / 2u;
-            if (s.tilesBefore(mr, mid, p.group) <= in) lo = mid;
+            if (unitsBefore(mid, p.group) <= in) lo = mid;
             else hi = mid - 1u;
         }
         item = lo;
-        item0 = base + kvHead * per + s.tilesBefore(mr, item, p.group);
+        item0 = base + kvHead * per + unitsBefore(item, p.group);
         tiles = s.tiles(mr, item, p.group);
-        return true;
+        return end - item0 > over;
     }
-    // Tiles [first, last) of the item are the block's.
-    __device__ __forceinline__ uint32_t first() const { return static_cast<uint32_t>(at - item0); }
-    __device__ __forceinline__ uint32_t last() const { return static_cast<uint32_t>(min(end - item0, static_cast<uint64_t>(tiles))); }
+    // Tiles [first, last) of the item are the block's; tiles of the item's first and last block.
+    __device__ __forceinline__ uint32_t first() const { return at - item0 > over ? static_cast<uint32_t>(at - item0 - over) : 0u; }
+    __device__ __forceinline__ uint32_t last() const { return static_cast<uint32_t>(min(end - item0, static_cast<uint64_t>(tiles) + over)) - over; }
+    __device__ __forceinline__ uint32_t firstBlock() const { return blockOf(item0 + over); }
+    __device__ __forceinline__ uint32_t lastBlock() const { return blockOf(item0 + over + tiles - 1u); }
     // On to the next item; false: the run is done.
     __device__ __forceinline__ bool next(const PagedAttnParams &p) {
-        item0 += tiles;
+        item0 += tiles + over;
         at = item0;
-        if (at >= end) return false;
+        if (at + over >= end) return false;  // (a run that ends in front of an item's tiles leaves it to the next block)
         if (++item == s.items(mr)) {
             item = 0;
             if (++kvHead == p.c.nKV) {

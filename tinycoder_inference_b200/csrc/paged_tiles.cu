@@ -2,7 +2,8 @@
 // accumulation in TMEM): chunks of prompts and whole prompts.
 //
 // The block is prefill_f16.cu's: two 128-row query tiles A and B share a ring of 64-row K and V tiles, warps 0-3 / 4-7 hold the softmax of
-// A / B a thread per row, warp 8 requests, warps 9, 10 issue S = Q K^T and warps 11, 12 O += P V with P in TMEM over the scores' buffer.
+// A / B a thread per row, warp 8 requests (fp16 V: warp 13), warps 9, 10 issue S = Q K^T and warps 11, 12 O += P V with P in TMEM over the
+// scores' buffer.
 // What differs is what a tile is and where it comes from:
 //   * a query tile holds tileTokens tokens x the q heads of one kv head (row = token x group + head; one TMA box), so a
 //     pass over the cache serves all of them and the causal edge is tileTokens rows wide instead of 128;
@@ -21,6 +22,10 @@ namespace tc {
 
 constexpr int kPtScales = 132;          // f32 of a scale slot: K's 64, V's 64, the power of two above V's; padding
 constexpr uint32_t kPtScaleSlots = 16;
+#ifndef PT_OVER
+#define PT_OVER 2
+#endif
+constexpr uint32_t kPtOver = PT_OVER;
 constexpr int kPtBN = int(kPaTile);
 constexpr float kPtLazyLog2 = 8.0f;  // O is rescaled when the row's maximum ran ahead by 2^8
 constexpr float kPtOff = 6.0f;       // probabilities are held as 2^6 p, at most 2^14: what fp16 has above them goes to the small ones
@@ -61,7 +66,7 @@ __device__ __forceinline__ PtItem ptItem(const PagedAttnParams &p, const PagedWa
     it.seq = w.seq, it.kvHead = w.kvHead, it.token0 = w.s.token0, it.len = w.s.len, it.before = w.s.before;
     it.part = 0, joins = 0, it.pad = 0;
     if (!it.whole) {
-        const uint32_t c0 = w.blockOf(w.item0), c1 = w.blockOf(w.item0 + w.tiles - 1u);
+        const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
         it.part = blockIdx.x == c0 ? 1u : 0u;
         if (blockIdx.x == c0) joins = c1 - c0 + 1u;
     }
@@ -70,7 +75,7 @@ __device__ __forceinline__ PtItem ptItem(const PagedAttnParams &p, const PagedWa
 
 template <int HD, bool I8>
 struct PtL {
-    static constexpr int kThreads = I8 ? 512 : 416;
+    static constexpr int kThreads = I8 ? 512 : 448;
     static constexpr int kHalves = HD / 64;
     static constexpr int kQTiles = HD > 128 ? 1 : 2;
     static constexpr int NK = HD > 128 ? 2 : I8 ? 3 : 6, NV = HD > 128 ? 2 : I8 ? 3 : 4;
@@ -165,13 +170,79 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         return pfWait<kCall>(&itemFull[n % kPtItems], (n / kPtItems) & 1u, err, kDevErrFullWait) && it->nTiles != 0u;
     };
 
+    // ---- requests: a copy per box of a tile, by the lanes side by side ----
+    // Where this lane's box of tile j lies.  Looked up a tile ahead of its first use: a request that waits for its table entry falls
+    // behind the products.
+    struct At {
+        uint32_t have, in;
+        int32_t page;
+    };
+    const uint32_t boxes = BN / p.box, boxBytes = p.box * 128u;
+    auto tableOf = [&](const PtItem &it) { return p.c.pages + static_cast<size_t>(it.seq) * p.c.pagesPerSeq; };
+    auto look = [&](const PtItem &it, const int32_t *table, uint32_t j) {
+        const uint32_t row0 = (it.t0 + j) * BN;
+        At at{it.len > row0 ? min(boxes, (it.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
+        if (lane < at.have) {
+            const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
+            at.in = row - slot * p.c.pageRows;
+            at.page = __ldg(table + slot);
+        }
+        return at;
+    };
+    auto pageOf = [&](const At &at) {
+        uint32_t page = static_cast<uint32_t>(at.page);
+        if (lane < at.have && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
+            atomicOr(err, kDevErrRowBound);
+            page = 0;
+        }
+        return page;
+    };
+    // an item's tiles of K or V, fp16
+    auto requestTiles = [&](const PtItem &it, const CUtensorMap *map, uint32_t base, uint64_t *full, uint64_t *empty, uint32_t &g, uint32_t N) {
+        const int32_t *table = tableOf(it);
+        At next = look(it, table, 0);
+        for (uint32_t j = 0; j < it.nTiles; ++j, ++g) {
+            const At at = next;
+            next = look(it, table, j + 1u);
+            const uint32_t page = pageOf(at), s = g % N;
+            if (g >= N && !pfWait<kCall>(&empty[s], ((g / N) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
+            if (lane == 0) mbarExpectTx(&full[s], at.have * boxBytes * L::kHalves);
+            __syncwarp();
+            if (lane < at.have) {
+#pragma unroll
+                for (int h = 0; h < L::kHalves; ++h)
+                    tmaLoad4D(smem + base + s * L::kKvTile + h * L::kKvHalf + lane * boxBytes, map, &full[s], 64 * h, it.kvHead, at.in, page);
+            }
+        }
+        return true;
+    };
+    // the panels of one tile, int8
+    auto requestPanels = [&](const PtItem &it, const At &at, const CUtensorMap *map, uint32_t &gs) {
+        const uint32_t page = pageOf(at);
+#pragma unroll
+        for (int h = 0; h < L::kPanels; ++h, ++gs) {
+            const uint32_t s = gs % (NS ? NS : 1u);
+            if (gs >= NS && !pfWait<kCall>(&stEmpty[s], ((gs / (NS ? NS : 1u)) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
+            if (lane == 0) mbarExpectTx(&stFull[s], at.have * boxBytes);
+            __syncwarp();
+            if (lane < at.have) tmaLoad4D(smem + L::kStaging + s * L::kKvHalf + lane * boxBytes, map, &stFull[s], 128 * h, it.kvHead, at.in, page);
+        }
+        return true;
+    };
+    // The last release of every slot has to have arrived before the block leaves; where somebody gave up, the copies under way
+    // still have to land.
+    auto drain = [&](uint64_t *bar, uint32_t count, uint32_t N, uint32_t bit) {
+        for (uint32_t back = 1; back <= N && back <= count; ++back)
+            if (!pfWait<kCall>(&bar[(count - back) % N], ((count - back) / N) & 1u, err, bit)) return false;
+        return true;
+    };
+
     if (warp == 8) {
         // ------------------------------- producer -------------------------------
-        uint32_t gk = 0, gv = 0, gs = 0, n = 0;
-        const uint32_t boxes = BN / p.box, boxBytes = p.box * 128u;
+        uint32_t gk = 0, gs = 0, n = 0;
         if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
         PagedWalk w;
-        const bool some = w.begin(p, tileRows * L::kQTiles);
+        const bool some = w.begin(p, tileRows * L::kQTiles, kPtOver);
         bool ok = true;
         if (some) do {
             uint32_t joins;
@@ -182,56 +253,6 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 if (joins != 0u) pagedLeaveJoin(p, &w, joins);
             }
             ++n;
-            const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
-            // Where this lane's box of tile j lies.  Looked up a tile ahead of its first use: a request that waits for its table entry
-            // falls behind the products.
-            struct At {
-                uint32_t have, in;
-                int32_t page;
-            };
-            auto look = [&](uint32_t j) {
-                const uint32_t row0 = (it.t0 + j) * BN;
-                At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
-                if (lane < at.have) {
-                    const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
-                    at.in = row - slot * p.c.pageRows;
-                    at.page = __ldg(table + slot);
-                }
-                return at;
-            };
-            auto request = [&](const At &at, const CUtensorMap *map, uint32_t base, uint64_t *full, uint64_t *empty, uint32_t &g, uint32_t N) {
-                const uint32_t have = at.have, in = at.in;
-                uint32_t page = static_cast<uint32_t>(at.page);
-                if (lane < have && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
-                    atomicOr(err, kDevErrRowBound);
-                    page = 0;
-                }
-                if constexpr (I8) {  // panel by panel to the converters
-#pragma unroll
-                    for (int h = 0; h < L::kPanels; ++h, ++gs) {
-                        const uint32_t s = gs % (NS ? NS : 1u);
-                        if (gs >= NS && !pfWait<kCall>(&stEmpty[s], ((gs / (NS ? NS : 1u)) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
-                        if (lane == 0) mbarExpectTx(&stFull[s], have * boxBytes);
-                        __syncwarp();
-                        if (lane < have) tmaLoad4D(smem + L::kStaging + s * L::kKvHalf + lane * boxBytes, map, &stFull[s], 128 * h, w.kvHead, in, page);
-                    }
-                    return true;
-                }
-                const uint32_t s = g % N;
-                if (g >= N && !pfWait<kCall>(&empty[s], ((g / N) - 1u) & 1u, err, kDevErrEmptyWait)) return false;
-                if (lane == 0) mbarExpectTx(&full[s], have * boxBytes * L::kHalves);
-                __syncwarp();
-                if (lane < have) {
-#pragma unroll
-                    for (int h = 0; h < L::kHalves; ++h)
-                        tmaLoad4D(smem + base + s * L::kKvTile + h * L::kKvHalf + lane * boxBytes, map, &full[s], 64 * h, w.kvHead, in, page);
-                }
-                ++g;
-                return true;
-            };
-            auto requestK = [&](const At &at) { return request(at, &tmK, L::kK, kFull, kEmpty, gk, NK); };
-            auto requestV = [&](const At &at) { return request(at, &tmV, L::kV, vFull, vEmpty, gv, NV); };
-            At a0 = look(0), a1 = look(1), a2 = look(2);  // tiles j, j + 1, j + 2 (rows past the run's last tile are only looked up)
             // the query tiles are free once the last score products of the previous item are complete
             if (n > 1u)
                 ok = pfWait<kCall>(&qFree[0], n & 1u, err, kDevErrEmptyWait) && (kOne || pfWait<kCall>(&qFree[1], n & 1u, err, kDevErrEmptyWait));
@@ -246,30 +267,39 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                                   w.s.token0 + it.m0 / p.group + x * p.tileTokens);
             }
             __syncwarp();
-            ok = requestK(a0) && (it.nTiles < 2u || requestK(a1));
-            for (uint32_t j = 0; ok && j < it.nTiles; ++j) {
-                const At a3 = look(j + 3u);
-                ok = (j + 2u >= it.nTiles || requestK(a2)) && requestV(a0);
-                a0 = a1, a1 = a2, a2 = a3;
+            if constexpr (I8) {  // K two tiles ahead of V, panel by panel to the converters
+                const int32_t *table = tableOf(it);
+                At a0 = look(it, table, 0), a1 = look(it, table, 1), a2 = look(it, table, 2);
+                ok = requestPanels(it, a0, &tmK, gs) && (it.nTiles < 2u || requestPanels(it, a1, &tmK, gs));
+                for (uint32_t j = 0; ok && j < it.nTiles; ++j) {
+                    const At a3 = look(it, table, j + 3u);
+                    ok = (j + 2u >= it.nTiles || requestPanels(it, a2, &tmK, gs)) && requestPanels(it, a0, &tmV, gs);
+                    a0 = a1, a1 = a2, a2 = a3;
+                }
+            } else {
+                ok = requestTiles(it, &tmK, L::kK, kFull, kEmpty, gk, NK);
             }
         } while (ok && w.next(p));
         if (lane == 0) {
             items[n % kPtItems].nTiles = 0u;
             mbarArrive(&itemFull[n % kPtItems]);
         }
-        // The last release of every slot has to have arrived before the block leaves; where somebody gave up, the copies under way
-        // still have to land.
-        auto drain = [&](uint64_t *bar, uint32_t count, uint32_t N, uint32_t bit) {
-            for (uint32_t back = 1; back <= N && back <= count; ++back)
-                if (!pfWait<kCall>(&bar[(count - back) % N], ((count - back) / N) & 1u, err, bit)) return false;
-            return true;
-        };
+        if (!ok && n != 0u) pfWait<kCall>(qFull, (n - 1u) & 1u, err, kDevErrFullWait);
         if constexpr (I8) {
             if (!ok || !drain(stEmpty, gs, NS ? NS : 1u, kDevErrEmptyWait)) drain(stFull, gs, NS ? NS : 1u, kDevErrFullWait);
-        } else if (!ok || !drain(kEmpty, gk, NK, kDevErrEmptyWait) || !drain(vEmpty, gv, NV, kDevErrEmptyWait)) {
+        } else if (!ok || !drain(kEmpty, gk, NK, kDevErrEmptyWait)) {
             drain(kFull, gk, NK, kDevErrFullWait);
-            drain(vFull, gv, NV, kDevErrFullWait);
         }
+    } else if (!I8 && warp == 13) {
+        // ---------------------- producer of V (page by page, one warp's requests are late) ----------------------
+        uint32_t gv = 0;
+        bool ok = true;
+        const PtItem *at;
+        for (uint32_t n = 0; ok && takeItem(n, at); ++n) {
+            const PtItem it = *at;
+            ok = requestTiles(it, &tmV, L::kV, vFull, vEmpty, gv, NV);
+        }
+        if (!ok || !drain(vEmpty, gv, NV, kDevErrEmptyWait)) drain(vFull, gv, NV, kDevErrFullWait);
     } else if (I8 && warp >= 13) {
         // ------------------------------ converters -----------------------------------
         // Panels of 64 rows x 128 int8 in the order of the producer's requests, one warp each in turn, into two fp16 halves: rows of 64 dims
@@ -337,7 +367,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             ok = convert(0, true) && (it.nTiles < 2u || convert(1, true));
             for (uint32_t j = 0; ok && j < it.nTiles; ++j) ok = (j + 2u >= it.nTiles || convert(j + 2u, true)) && convert(j, false);
         }
-    } else if (warp >= 9) {
+    } else if (warp >= 9 && warp < 13) {
         // ------------------------------- MMA issuers -------------------------------
         // t counts the tiles of X over all items; tile t uses score buffer t % 2, which P(t - 2) has to have left (kAhead: the softmax
         // threads have to have read S(t - 1)).  A tile that is not X's is released all the same, once it is there: a warp that ran ahead would
