@@ -28,7 +28,10 @@ namespace tc {
 #ifndef PA_OVER
 #define PA_OVER 0
 #endif
-constexpr uint32_t kPaOver = PA_OVER;
+#ifndef PA_RUN
+#define PA_RUN 1
+#endif
+constexpr uint32_t kPaOver = PA_OVER, kPaRun = PA_RUN;
 constexpr int kPaThreads = 160;       // four consumer warps, one producer warp
 // The workspace: two partials per block of the two kernels' widest grids, then what the merge finds per block.
 constexpr size_t kRowsParts = size_t(2) * kPagedSMs * 2 * pagedSlot(64, 128);       // f32
@@ -193,7 +196,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     gridDepLaunch();
     PagedWalk w;
     if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
-    if (!w.begin(p, MR, kPaOver)) return;
+    if (!w.begin(p, MR, kPaOver, kPaRun)) return;
     bool ok = true;
     uint32_t g = 0;  // tiles so far
 
@@ -705,7 +708,7 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
         const int rb = pagedAttnTiles(c, b, st);
         if (rb != TC_OK) return rb;
     }
-    const dim3 grid(blocksA + (tiles ? std::min(numSMs(), kPagedSMs) : 0), tiles ? 32 : 8);
+    const dim3 grid(blocksA + (tiles ? std::min(numSMs(), kPagedSMs) : 0), 8);
     auto merge = c->hd == 64 ? pagedMergeKernel<64> : c->hd == 128 ? pagedMergeKernel<128> : pagedMergeKernel<256>;
     return launchDependent(merge, grid, 256, 0, st, 1, p, static_cast<const float *>(partsB), static_cast<const PagedJoin *>(joinsB), blocksA);
 }

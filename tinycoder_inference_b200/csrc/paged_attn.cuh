@@ -37,17 +37,39 @@ struct PagedAttnParams {
 };
 
 #ifdef __CUDACC__
-// sum of (a i + b) / m over i = 0 .. n - 1, rounded down each
-__device__ __forceinline__ uint64_t floorSum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+// Quotients of numbers that are small as a rule: a 64-bit division takes some hundred cycles, and a block starts with a chain of them.
+__device__ __forceinline__ uint64_t divide(uint64_t a, uint64_t b) {
+    return ((a | b) >> 32) == 0u ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
+}
+// sum of (a i + b) / m over i = 0 .. n - 1, rounded down each: term by term while there are few, else by Euclid's steps on (a, m)
+__device__ __forceinline__ uint64_t floorSum(uint32_t n, uint32_t m, uint32_t a, uint64_t b0) {
     uint64_t sum = 0;
+    if (n <= 24u) {
+        const uint64_t q0 = divide(b0, m);
+        uint32_t r = static_cast<uint32_t>(b0 - q0 * m), q = 0, part = 0;
+        const uint32_t qa = a / m, ra = a - qa * m;
+        for (uint32_t i = 0; i < n; ++i) {
+            part += q;
+            r += ra, q += qa;
+            if (r >= m) r -= m, ++q;
+        }
+        return q0 * n + part;
+    }
+    uint64_t nn = n, mm = m, aa = a, b = b0;
     for (;;) {
-        if (a >= m) sum += n * (n - 1) / 2 * (a / m), a %= m;
-        if (b >= m) sum += n * (b / m), b %= m;
-        const uint64_t top = a * n + b;
-        if (top < m) return sum;
-        n = top / m, b = top % m;
-        const uint64_t x = m;
-        m = a, a = x;
+        if (aa >= mm) {
+            const uint64_t q = divide(aa, mm);
+            sum += nn * (nn - 1) / 2 * q, aa -= q * mm;
+        }
+        if (b >= mm) {
+            const uint64_t q = divide(b, mm);
+            sum += nn * q, b -= q * mm;
+        }
+        const uint64_t top = aa * nn + b;
+        if (top < mm) return sum;
+        nn = divide(top, mm), b = top - nn * mm;
+        const uint64_t x = mm;
+        mm = aa, aa = x;
     }
 }
 
@@ -77,7 +99,7 @@ struct PagedSeq {
         const uint32_t n = all ? m - 1u : m;
         uint64_t sum = all ? tiles(MR, m - 1u, group) : 0u;
         // item i sees before + ((i + 1) MR - 1) / group + 1 rows: floor((group (before + kPaTile) + (i + 1) MR - 1) / (kPaTile group)) tiles
-        if (n > 0u) sum += floorSum(n, static_cast<uint64_t>(kPaTile) * group, MR, static_cast<uint64_t>(group) * (static_cast<uint32_t>(before) + kPaTile) + MR - 1u);
+        if (n > 0u) sum += floorSum(n, kPaTile * group, MR, static_cast<uint64_t>(group) * (static_cast<uint32_t>(before) + kPaTile) + MR - 1u);
         return sum;
     }
     __device__ __forceinline__ uint64_t tilesAll(uint32_t MR, uint32_t group) const { return rows == 0u ? 0u : tilesBefore(MR, items(MR), group); }
@@ -110,31 +132,31 @@ struct PagedWalk {
     uint32_t tiles;           // its tiles
     PagedSeq s;
 
-    __device__ __forceinline__ uint64_t firstOf(uint32_t block) const { return static_cast<uint64_t>(block) * total / blocks; }
-    __device__ __forceinline__ uint32_t blockOf(uint64_t unit) const { return static_cast<uint32_t>(((unit + 1u) * blocks - 1u) / total); }
+    __device__ __forceinline__ uint64_t firstOf(uint32_t block) const { return divide(block * total, blocks); }
+    __device__ __forceinline__ uint32_t blockOf(uint64_t unit) const { return static_cast<uint32_t>(divide((unit + 1u) * blocks - 1u, total)); }
 
     __device__ __forceinline__ uint64_t unitsAll(const PagedSeq &q, uint32_t group) const { return q.tilesAll(mr, group) + static_cast<uint64_t>(over) * q.items(mr); }
     __device__ __forceinline__ uint64_t unitsBefore(uint32_t m, uint32_t group) const { return s.tilesBefore(mr, m, group) + static_cast<uint64_t>(over) * m; }
 
-    // All lanes of the warp.  False: nothing to do.
-    __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
+    // All lanes of the warp.  False: nothing to do.  leastRun: units that a block has at least, where there are so many.
+    __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead, uint32_t leastRun) {
         mr = itemRows, over = overhead;
         const uint32_t lane = threadIdx.x & 31u;
-        uint64_t sum = 0;
-        for (uint32_t b0 = 0; b0 < p.c.batch; b0 += 32u)
-            if (b0 + lane < p.c.batch) sum += unitsAll(pagedSeq(p, b0 + lane), p.group) * p.c.nKV;
+        auto unitsOf = [&](uint32_t b) { return b < p.c.batch ? unitsAll(pagedSeq(p, b), p.group) * p.c.nKV : 0u; };
+        const uint64_t lead = unitsOf(lane);  // of the first 32 sequences
+        uint64_t sum = lead;
+        for (uint32_t b0 = 32u; b0 < p.c.batch; b0 += 32u) sum += unitsOf(b0 + lane);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum;
         if (total == 0u) return false;
-        blocks = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x), total));
+        blocks = static_cast<uint32_t>(max(static_cast<uint64_t>(1), min(static_cast<uint64_t>(gridDim.x), divide(total, leastRun))));
         if (blockIdx.x >= blocks) return false;
         at = firstOf(blockIdx.x), end = firstOf(blockIdx.x + 1u);
         // the sequence that holds unit `at`
         uint64_t base = 0;
         for (uint32_t b0 = 0;; b0 += 32u) {
-            uint64_t mine = 0;
-            if (b0 + lane < p.c.batch) mine = unitsAll(pagedSeq(p, b0 + lane), p.group) * p.c.nKV;
+            const uint64_t mine = b0 == 0u ? lead : unitsOf(b0 + lane);
             uint64_t upTo = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -152,17 +174,23 @@ struct PagedWalk {
             if (b0 + 32u >= p.c.batch) return false;  // (not reached: `at` lies below the sum)
         }
         s = pagedSeq(p, seq);
-        const uint64_t per = unitsAll(s, p.group);
-        kvHead = static_cast<uint32_t>((at - base) / per);
-        const uint64_t in = at - base - kvHead * per;
-        uint32_t lo = 0, hi = s.items(mr) - 1u;  // the last item whose first tile is not behind `in`
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi + 1u) / 2u;
-            if (unitsBefore(mid, p.group) <= in) lo = mid;
-            else hi = mid - 1u;
+        uint64_t in = at - base;
+        kvHead = 0;
+        if (p.c.nKV > 1u) {
+            const uint64_t per = unitsAll(s, p.group);
+            kvHead = static_cast<uint32_t>(divide(in, per));
+            in -= kvHead * per;
+        }
+        // the last item that does not begin behind `in`, 32 candidates at a time
+        uint32_t lo = 0, n = s.items(mr);
+        while (n > 1u) {
+            const uint32_t step = (n + 31u) / 32u, try_ = lo + lane * step;
+            const uint32_t hits = __popc(__ballot_sync(0xffffffffu, lane * step < n && unitsBefore(try_, p.group) <= in));
+            lo += (hits - 1u) * step;
+            n = min(step, n - (hits - 1u) * step);
         }
         item = lo;
-        item0 = base + kvHead * per + unitsBefore(item, p.group);
+        item0 = at - in + unitsBefore(item, p.group);
         tiles = s.tiles(mr, item, p.group);
         return end - item0 > over;
     }

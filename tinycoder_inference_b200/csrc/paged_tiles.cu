@@ -25,7 +25,10 @@ constexpr uint32_t kPtScaleSlots = 16;
 #ifndef PT_OVER
 #define PT_OVER 2
 #endif
-constexpr uint32_t kPtOver = PT_OVER;
+#ifndef PT_RUN
+#define PT_RUN 1
+#endif
+constexpr uint32_t kPtOver = PT_OVER, kPtRun = PT_RUN;
 constexpr int kPtBN = int(kPaTile);
 constexpr float kPtLazyLog2 = 8.0f;  // O is rescaled when the row's maximum ran ahead by 2^8
 constexpr float kPtOff = 6.0f;       // probabilities are held as 2^6 p, at most 2^14: what fp16 has above them goes to the small ones
@@ -242,7 +245,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         uint32_t gk = 0, gs = 0, n = 0;
         if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
         PagedWalk w;
-        const bool some = w.begin(p, tileRows * L::kQTiles, kPtOver);
+        const bool some = w.begin(p, tileRows * L::kQTiles, kPtOver, kPtRun);
         bool ok = true;
         if (some) do {
             uint32_t joins;
