@@ -32,7 +32,6 @@ namespace tc {
 #define PA_RUN 1
 #endif
 constexpr uint32_t kPaOver = PA_OVER, kPaRun = PA_RUN;
-constexpr int kPaThreads = 160;       // four consumer warps, one producer warp
 // The workspace: two partials per block of the two kernels' widest grids, then what the merge finds per block.
 constexpr size_t kRowsParts = size_t(2) * kPagedSMs * 2 * pagedSlot(64, 128);       // f32
 constexpr size_t kTilesParts = size_t(2) * kPagedSMs * pagedSlot(2 * kPagedTile, 128);
@@ -40,9 +39,22 @@ static_assert(2 * pagedSlot(64, 128) >= pagedSlot(64, 256) && pagedSlot(2 * kPag
 constexpr size_t kPagedWorkspace = (kRowsParts + kTilesParts) * 4 + size_t(kPagedSMs) * 3 * sizeof(PagedJoin) + 32;
 constexpr float kPaOff = 13.0f;       // p is held as 2^13 p: its fp16 pair keeps 11 + 11 bits down to p = 2^-27
 
+// What a block has of an item, as its producer hands it to the consumers: tiles t0 .. t0 + nTiles - 1 of it (nTiles 0: the run is
+// done), query rows m0 .. of `rows`.
+struct PaItem {
+    uint32_t nTiles, t0, m0, rows, token0, kvHead, len, whole, part;
+    int32_t before;
+};
+constexpr uint32_t kPaItems = 8;  // the ring's stages and two: a consumer may still write the results of an item whose tiles are all released
+
 template <int HD, bool I8, bool PAIR, int WM>
 struct PaL {
-    static constexpr int WK = 4 / WM, KS = int(kPaTile) / WK;       // shares of a tile; rows of a share
+    static constexpr int NW = HD == 256 && WM > 1 ? 8 : 4;          // consumer warps; a producer beside them
+    // 8 consumer warps: a warpgroup for the producer, whose registers go to theirs (232 x 256 + 40 x 128 = 168 x 384, what the block is
+    // launched with)
+    static constexpr bool kSplitRegs = NW == 8;
+    static constexpr int kThreads = kSplitRegs ? 384 : 32 * (NW + 1);
+    static constexpr int WK = NW / WM, KS = int(kPaTile) / WK;      // shares of a tile; rows of a share
     static constexpr int RW = PAIR ? 8 : 16;                       // query rows of a warp
     static constexpr int MR = WM * RW;
     static constexpr int kPanels = HD * (I8 ? 1 : 2) / 128;        // 128-byte columns of a row
@@ -53,9 +65,11 @@ struct PaL {
     static constexpr int NST = HD == 256 ? (I8 ? 6 : 3) : (kStage == 16384 ? 5 : 3);
     static constexpr int kScales = NST * kStage;                   // [stage][K, V][64]
     static constexpr int kBuf = kScales + (I8 ? NST * 512 : 0);    // [warp][16][36] f32
-    static constexpr int kMl = kBuf + 4 * 16 * 36 * 4;             // [warp][16] (m, l)
-    static constexpr int kBars = kMl + 4 * 16 * 8;
-    static constexpr int kTotal = kBars + 2 * NST * 8 + 1024;
+    static constexpr int kMl = kBuf + NW * 16 * 36 * 4;            // [warp][16] (m, l)
+    static constexpr int kItems = kMl + NW * 16 * 8;
+    static constexpr int kBars = kItems + int(kPaItems * sizeof(PaItem));
+    static constexpr int kTotal = kBars + (2 * NST + int(kPaItems)) * 8 + 1024;
+    static_assert(NST + 2 <= int(kPaItems), "items");
     static constexpr int kBlocks = HD == 256 ? 1 : 2;
     static_assert(kBlocks * (kTotal + 1024) <= 228 * 1024, "shared memory of an SM");
 };
@@ -174,19 +188,21 @@ __global__ void __launch_bounds__(256) pagedMergeKernel(const __grid_constant__ 
 }
 
 template <int HD, bool I8, bool PAIR, int WM>
-__global__ void __launch_bounds__(kPaThreads, (PaL<HD, I8, PAIR, WM>::kBlocks))
+__global__ void __launch_bounds__((PaL<HD, I8, PAIR, WM>::kThreads), (PaL<HD, I8, PAIR, WM>::kBlocks))
 pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedAttnParams p) {
     using L = PaL<HD, I8, PAIR, WM>;
     constexpr uint32_t NST = L::NST, MR = L::MR, WK = L::WK;
     extern __shared__ uint8_t smemRaw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kBars), *empty = full + NST;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kBars), *empty = full + NST, *itemFull = empty + NST;
+    PaItem *items = reinterpret_cast<PaItem *>(smem + L::kItems);
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < NST; ++i) {
             mbarInit(&full[i], I8 ? 33 : 1);  // (int8: every lane of the producer brings scales)
-            mbarInit(&empty[i], 4);
+            mbarInit(&empty[i], L::NW);
         }
+        for (uint32_t i = 0; i < kPaItems; ++i) mbarInit(&itemFull[i], 1);
         fenceBarrierInit();
         tmaPrefetchDesc(&tmK);
         tmaPrefetchDesc(&tmV);
@@ -194,18 +210,37 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     __syncthreads();
     gridDepWait();
     gridDepLaunch();
-    PagedWalk w;
-    if (threadIdx.x == 0) pagedLeaveJoin(p, nullptr, 0u);
-    if (!w.begin(p, MR, kPaOver, kPaRun)) return;
-    bool ok = true;
     uint32_t g = 0;  // tiles so far
+    if constexpr (L::kSplitRegs) {
+        if (warp >= L::NW) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        if (warp > L::NW) return;
+    }
 
-    if (warp == 4) {
+    if (warp == L::NW) {
         // ------------------------------- producer -------------------------------
         const uint32_t boxes = kPaTile / p.box, boxBytes = p.box * 128u;
-        do {
+        if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
+        PagedWalk w;
+        uint32_t handed = 0;  // items
+        bool ok = true;
+        if (w.begin(p, MR, kPaOver, kPaRun)) do {
             const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
             const uint32_t t1 = w.last();
+            if (lane == 0) {
+                PaItem it;
+                it.t0 = w.first(), it.nTiles = t1 - it.t0, it.m0 = w.item * MR, it.rows = w.s.rows, it.token0 = w.s.token0;
+                it.kvHead = w.kvHead, it.len = w.s.len, it.before = w.s.before;
+                it.whole = it.t0 == 0u && t1 == w.tiles, it.part = 0;
+                if (!it.whole) {
+                    const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
+                    it.part = blockIdx.x == c0 ? 1u : 0u;
+                    if (it.part) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
+                }
+                items[handed % kPaItems] = it;
+                mbarArrive(&itemFull[handed % kPaItems]);
+            }
+            ++handed;
             // where this lane's box of a tile lies: looked up a tile ahead
             struct At {
                 uint32_t have, in;
@@ -259,6 +294,10 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 }
             }
         } while (ok && w.next(p));
+        if (lane == 0) {
+            items[handed % kPaItems].nTiles = 0u;
+            mbarArrive(&itemFull[handed % kPaItems]);
+        }
         // no copy is under way any more when the block leaves
         for (uint32_t back = 1; back <= NST && back <= g; ++back)
             if (!pfWait<true>(&full[(g - back) % NST], ((g - back) / NST) & 1u, p.c.err, kDevErrFullWait)) break;
@@ -280,17 +319,22 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         if (WK == 1) __syncwarp();
         else namedBarSync(1u + wm, WK * 32u);
     };
-    do {
+    bool ok = true;  // (a warp that gave up still takes its items and meets the others at their barriers)
+    for (uint32_t n = 0;; ++n) {
+        // The producer hands in the end of the run whatever becomes of its waits, each of which is bounded: this one only has to be longer.
+        for (uint32_t i = 0; i < (1u << 20) && !mbarTryWait(&itemFull[n % kPaItems], (n / kPaItems) & 1u); ++i) {}
+        const PaItem it = items[n % kPaItems];
+        if (it.nTiles == 0u) break;
         // q as A operands
         uint32_t qa[NS][4];
         float rowScale[NR];
         int32_t vis[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const uint32_t rr = w.item * MR + wm * L::RW + n8 + 8u * r;
-            const bool valid = rr < w.s.rows;
-            const uint32_t tok = w.s.token0 + rr / p.group, head = w.kvHead * p.group + rr % p.group;
-            vis[r] = valid ? w.s.before + static_cast<int32_t>(rr / p.group) + 1 : 0;
+            const uint32_t rr = it.m0 + wm * L::RW + n8 + 8u * r;
+            const bool valid = rr < it.rows;
+            const uint32_t tok = it.token0 + rr / p.group, head = it.kvHead * p.group + rr % p.group;
+            vis[r] = valid ? it.before + static_cast<int32_t>(rr / p.group) + 1 : 0;
             rowScale[r] = p.scaleLog2;
             const size_t base = (static_cast<size_t>(tok) * p.nHeads + head) * HD;
             auto dim = [&](int st) { return I8 ? 128 * (st / 8) + 32 * static_cast<int>(c) + 4 * (st % 8) : 64 * (st / 4) + 16 * static_cast<int>(c) + 4 * (st % 4); };
@@ -344,14 +388,14 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < OR; ++e) o[j][e] = 0.0f;
 
-        const uint32_t t0 = w.first(), t1 = w.last();
+        const uint32_t t0 = it.t0, t1 = t0 + it.nTiles;
         for (uint32_t t = t0; t < t1; ++t, ++g) {
             const uint32_t st = g % NST;
             ok = ok && pfWait<true>(&full[st], (g / NST) & 1u, p.c.err, kDevErrFullWait);
             if (!ok) break;
             const uint32_t sK = smemAddr(smem + st * L::kStage), sV = sK + L::kMat;
             const float *sc = reinterpret_cast<const float *>(smem + L::kScales) + st * 128u;
-            const int32_t left = static_cast<int32_t>(w.s.len) - static_cast<int32_t>(t * kPaTile);  // rows of the tile that exist
+            const int32_t left = static_cast<int32_t>(it.len) - static_cast<int32_t>(t * kPaTile);  // rows of the tile that exist
             float s[NT][2 * NR];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -518,7 +562,6 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             __syncwarp();
             if (lane == 0) mbarArrive(&empty[st]);
         }
-        // (a warp that gave up still takes part in what follows: the others wait for it there)
         // ---- the shares of a row group, then the blocks of the item ----
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -543,9 +586,8 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 for (uint32_t i = 0; i < WK; ++i) sum[r] = fmaf(fastExp2(x[i].x - (M[r] == -INFINITY ? 0.0f : M[r])), x[i].y, sum[r]);
             }
         }
-        const bool whole = t0 == 0u && t1 == w.tiles;
-        const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
-        float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + (blockIdx.x == c0 ? 1u : 0u)) * pagedSlot(MR, HD);
+        const bool whole = it.whole != 0u;
+        float *part = p.parts + (2u * static_cast<size_t>(blockIdx.x) + it.part) * pagedSlot(MR, HD);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const float Mu = M[r] == -INFINITY ? 0.0f : M[r];
@@ -581,15 +623,14 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
                 }
                 const uint32_t dim = I8 ? 128u * (pass / 4) + 16u * q4 + 4u * (pass % 4) : 32u * pass + 4u * q4;
-                const uint32_t local = wm * L::RW + row, r = w.item * MR + local;
-                if (r >= w.s.rows) continue;
-                if (whole) pagedStore(p, HD, w.s.token0, w.kvHead, r, dim, x);
+                const uint32_t local = wm * L::RW + row, r = it.m0 + local;
+                if (r >= it.rows) continue;
+                if (whole) pagedStore(p, HD, it.token0, it.kvHead, r, dim, x);
                 else __stcg(reinterpret_cast<float4 *>(part + local * HD + dim), x);
             }
         }
         groupSync();
-        if (threadIdx.x == 0 && !whole && blockIdx.x == c0) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
-    } while (w.next(p));
+    }
 }
 
 static uint32_t pagedRowsBlocks(uint32_t hd) { return std::min(numSMs(), kPagedSMs) * (hd == 256 ? 1 : 2); }
@@ -605,7 +646,7 @@ static int launchPagedRows(const CUtensorMap &k, const CUtensorMap &v, const Pag
         attrDone[dev] = true;
     }
     const uint32_t blocks = pagedRowsBlocks(HD);
-    return launchDependent(kern, dim3(blocks), kPaThreads, L::kTotal, st, 1, k, v, p);
+    return launchDependent(kern, dim3(blocks), L::kThreads, L::kTotal, st, 1, k, v, p);
 }
 
 int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v) {
