@@ -21,34 +21,14 @@
 #include <cstring>
 
 #include "paged_attn.cuh"
-#include "tc_tcgen05.cuh"
 
 namespace tc {
 
-#ifndef PA_OVER
-#define PA_OVER 0
-#endif
-#ifndef PA_RUN
-#define PA_RUN 1
-#endif
-constexpr uint32_t kPaOver = PA_OVER, kPaRun = PA_RUN;
-// The workspace: two partials per block of the two kernels' widest grids, then what the merge finds per block.
-constexpr size_t kRowsParts = size_t(2) * kPagedSMs * 2 * pagedSlot(64, 128);       // f32
-constexpr size_t kTilesParts = size_t(2) * kPagedSMs * pagedSlot(2 * kPagedTile, 128);
-static_assert(2 * pagedSlot(64, 128) >= pagedSlot(64, 256) && pagedSlot(2 * kPagedTile, 128) >= pagedSlot(kPagedTile, 256), "one block per SM at head_dim 256");
-constexpr size_t kPagedWorkspace = (kRowsParts + kTilesParts) * 4 + size_t(kPagedSMs) * 3 * sizeof(PagedJoin) + 32;
-constexpr float kPaOff = 13.0f;       // p is held as 2^13 p: its fp16 pair keeps 11 + 11 bits down to p = 2^-27
-
-// What a block has of an item, as its producer hands it to the consumers: tiles t0 .. t0 + nTiles - 1 of it (nTiles 0: the run is
-// done), query rows m0 .. of `rows`.
-struct PaItem {
-    uint32_t nTiles, t0, m0, rows, token0, kvHead, len, whole, part;
-    int32_t before;
-};
-constexpr uint32_t kPaItems = 8;  // the ring's stages and two: a consumer may still write the results of an item whose tiles are all released
+constexpr float kPaOff = 13.0f;  // p is held as 2^13 p: its fp16 pair keeps 11 + 11 bits down to p = 2^-27
 
 template <int HD, bool I8, bool PAIR, int WM>
 struct PaL {
+    static constexpr bool kI8 = I8;
     static constexpr int NW = HD == 256 && WM > 1 ? 8 : 4;          // consumer warps; a producer beside them
     // 8 consumer warps: a warpgroup for the producer, whose registers go to theirs (232 x 256 + 40 x 128 = 168 x 384, what the block is
     // launched with)
@@ -73,13 +53,6 @@ struct PaL {
     static constexpr int kBlocks = HD == 256 ? 1 : 2;
     static_assert(kBlocks * (kTotal + 1024) <= 228 * 1024, "shared memory of an SM");
 };
-
-__device__ __forceinline__ void pagedStore(const PagedAttnParams &p, uint32_t hd, uint32_t token0, uint32_t kvHead, uint32_t r, uint32_t dim, const float4 &x) {
-    const uint32_t tok = token0 + r / p.group, head = kvHead * p.group + r % p.group;
-    const size_t at = (static_cast<size_t>(tok) * p.nHeads + head) * hd + dim;
-    if (p.half) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + at) = make_uint2(packHalf2(x.x, x.y), packHalf2(x.z, x.w));
-    else *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = x;
-}
 
 // The partials of the items that several blocks had a part in: block (i, y) takes item i's rows y, y + gridDim.y, ... (in steps of 8 / W).
 // W warps share a row, each a W-th of its partials: few rows of many parts (a step of one long session: 74) are as much a chain of loads
@@ -218,89 +191,7 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     }
 
     if (warp == L::NW) {
-        // ------------------------------- producer -------------------------------
-        const uint32_t boxes = kPaTile / p.box, boxBytes = p.box * 128u;
-        if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
-        PagedWalk w;
-        uint32_t handed = 0;  // items
-        bool ok = true;
-        if (w.begin(p, MR, kPaOver, kPaRun)) do {
-            const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
-            const uint32_t t1 = w.last();
-            if (lane == 0) {
-                PaItem it;
-                it.t0 = w.first(), it.nTiles = t1 - it.t0, it.m0 = w.item * MR, it.rows = w.s.rows, it.token0 = w.s.token0;
-                it.kvHead = w.kvHead, it.len = w.s.len, it.before = w.s.before;
-                it.whole = it.t0 == 0u && t1 == w.tiles, it.part = 0;
-                if (!it.whole) {
-                    const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
-                    it.part = blockIdx.x == c0 ? 1u : 0u;
-                    if (it.part) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
-                }
-                items[handed % kPaItems] = it;
-                mbarArrive(&itemFull[handed % kPaItems]);
-            }
-            ++handed;
-            // where this lane's box of a tile lies: looked up a tile ahead
-            struct At {
-                uint32_t have, in;
-                int32_t page;
-            };
-            auto look = [&](uint32_t t) {
-                const uint32_t row0 = t * kPaTile;
-                At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
-                if (lane < at.have) {
-                    const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
-                    at.in = row - slot * p.c.pageRows;
-                    at.page = __ldg(table + slot);
-                }
-                return at;
-            };
-            At next = look(w.first());
-            for (uint32_t t = w.first(); t < t1; ++t, ++g) {
-                const uint32_t n = next.have, in = next.in;
-                uint32_t page = static_cast<uint32_t>(next.page);
-                next = look(t + 1u);
-                if (lane < n && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
-                    atomicOr(p.c.err, kDevErrRowBound);
-                    page = 0;
-                }
-                const uint32_t st = g % NST;
-                if (g >= NST) ok = pfWait<true>(&empty[st], ((g / NST) - 1u) & 1u, p.c.err, kDevErrEmptyWait);
-                if (!ok) break;
-                if (lane == 0) mbarExpectTx(&full[st], n * boxBytes * 2u * L::kPanels);
-                __syncwarp();
-                uint8_t *stage = smem + st * L::kStage;
-                if (lane < n) {
-#pragma unroll
-                    for (int h = 0; h < L::kPanels; ++h) {
-                        tmaLoad4D(stage + h * L::kPanel + lane * boxBytes, &tmK, &full[st], h * (I8 ? 128 : 64), w.kvHead, in, page);
-                        tmaLoad4D(stage + L::kMat + h * L::kPanel + lane * boxBytes, &tmV, &full[st], h * (I8 ? 128 : 64), w.kvHead, in, page);
-                    }
-                }
-                if constexpr (I8) {
-                    float *sc = reinterpret_cast<float *>(smem + L::kScales) + st * 128u;
-#pragma unroll
-                    for (uint32_t u = 0; u < 2; ++u) {
-                        const uint32_t key = lane + 32u * u, from = key / p.box;
-                        const uint32_t pg = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, in, from) + key - from * p.box;
-                        if (from < n) {
-                            const size_t at = (static_cast<size_t>(pg) * p.c.pageRows + r) * p.c.nKV + w.kvHead;
-                            cpAsync4(sc + key, p.ks + at);
-                            cpAsync4(sc + 64u + key, p.vs + at);
-                        }
-                    }
-                    cpAsyncMbarArriveNoinc(&full[st]);
-                }
-            }
-        } while (ok && w.next(p));
-        if (lane == 0) {
-            items[handed % kPaItems].nTiles = 0u;
-            mbarArrive(&itemFull[handed % kPaItems]);
-        }
-        // no copy is under way any more when the block leaves
-        for (uint32_t back = 1; back <= NST && back <= g; ++back)
-            if (!pfWait<true>(&full[(g - back) % NST], ((g - back) / NST) & 1u, p.c.err, kDevErrFullWait)) break;
+        pagedProduce<L>(p, tmK, tmV, smem, full, empty, itemFull, items);
         return;
     }
 
@@ -667,20 +558,19 @@ int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v
 }
 
 // rows: how many query rows per kv head a sequence brings as a rule, for the choice of a form; any number is right
-static int pagedAttnRows(const tc_paged_kv *c, const PagedAttnParams &p, uint32_t rows, cudaStream_t st) {
+static int pagedAttnRows(const tc_paged_kv *c, const PagedAttnParams &p, uint32_t rows, cudaStream_t st, uint32_t *blocks) {
+    if (rows <= pagedStepRows(c)) return pagedAttnSteps(c, p, rows, st, blocks);
     CUtensorMap k, v;
     const int rc = pagedMaps(c, p.box, &k, &v);
     if (rc != TC_OK) return rc;
-    const bool pair = !p.half || rows <= 8;
-    const int wm = pair ? (rows <= 8 ? 1 : rows <= 16 ? 2 : 4) : (rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
-#define TC_PAGED_WM(HD, I8, PAIR) \
-    (wm == 1 ? launchPagedRows<HD, I8, PAIR, 1>(k, v, p, st) : wm == 2 ? launchPagedRows<HD, I8, PAIR, 2>(k, v, p, st) : launchPagedRows<HD, I8, PAIR, 4>(k, v, p, st))
-#define TC_PAGED_PAIR(HD, I8) (pair ? TC_PAGED_WM(HD, I8, true) : TC_PAGED_WM(HD, I8, false))
-    if (c->kvI8) return c->hd == 128 ? TC_PAGED_PAIR(128, true) : TC_PAGED_PAIR(256, true);
-    if (c->hd == 64) return TC_PAGED_PAIR(64, false);
-    return c->hd == 128 ? TC_PAGED_PAIR(128, false) : TC_PAGED_PAIR(256, false);
-#undef TC_PAGED_PAIR
-#undef TC_PAGED_WM
+    *blocks = pagedRowsBlocks(c->hd);
+    const int wm = !p.half || rows > 32 ? 4 : 2;  // (f32 results: the forms of fewer rows are paged_steps.cu's)
+#define TC_PAGED_ROWS(HD, I8) \
+    (!p.half ? launchPagedRows<HD, I8, true, 4>(k, v, p, st) : wm == 2 ? launchPagedRows<HD, I8, false, 2>(k, v, p, st) : launchPagedRows<HD, I8, false, 4>(k, v, p, st))
+    if (c->kvI8) return c->hd == 128 ? TC_PAGED_ROWS(128, true) : TC_PAGED_ROWS(256, true);
+    if (c->hd == 64) return TC_PAGED_ROWS(64, false);
+    return c->hd == 128 ? TC_PAGED_ROWS(128, false) : TC_PAGED_ROWS(256, false);
+#undef TC_PAGED_ROWS
 }
 
 // Query rows per kv head from which on a call's sequences are tiles of the tensor cores; in such a call, what the rows kernel keeps.
@@ -722,7 +612,7 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
     p.parts = reinterpret_cast<float *>(base);
     float *const partsB = p.parts + kRowsParts;
     p.joins = reinterpret_cast<PagedJoin *>(partsB + kTilesParts);
-    PagedJoin *const joinsB = p.joins + 2 * kPagedSMs;
+    PagedJoin *const joinsB = p.joins + 3 * kPagedSMs;
     p.nHeads = nHeads, p.group = nHeads / c->nKV;
     p.box = 64;
     while (c->pageRows % p.box != 0) p.box /= 2;
@@ -738,9 +628,8 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
     uint32_t blocksA = 0;
     if (rowsToo) {
         p.minRows = 1, p.maxRows = tiles ? kRowsBeside : 0xffffffffu;
-        const int ra = pagedAttnRows(c, p, tiles ? kRowsBeside : rows, st);
+        const int ra = pagedAttnRows(c, p, tiles ? kRowsBeside : rows, st, &blocksA);
         if (ra != TC_OK) return ra;
-        blocksA = pagedRowsBlocks(c->hd);
     }
     if (tiles) {
         PagedAttnParams b = p;

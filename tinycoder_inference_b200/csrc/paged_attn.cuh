@@ -8,6 +8,7 @@
 #pragma once
 
 #include "paged.cuh"
+#include "tc_tcgen05.cuh"
 
 namespace tc {
 
@@ -239,12 +240,127 @@ __device__ __forceinline__ void pagedLeaveJoin(const PagedAttnParams &p, const P
     if (count != 0u) j.row0 = w->item * w->mr, j.rows = w->s.rows, j.token0 = w->s.token0, j.kvHead = w->kvHead, j.mr = w->mr;
     p.joins[blockIdx.x] = j;
 }
+// What a block has of an item, as its producer hands it to the consumers: tiles t0 .. t0 + nTiles - 1 of it (nTiles 0: the run is
+// done), query rows m0 .. of `rows`.
+struct PaItem {
+    uint32_t nTiles, t0, m0, rows, token0, kvHead, len, whole, part;
+    int32_t before;
+};
+constexpr uint32_t kPaItems = 8;  // the ring's stages and two: a consumer may still write the results of an item whose tiles are all released
+
+__device__ __forceinline__ void pagedStore(const PagedAttnParams &p, uint32_t hd, uint32_t token0, uint32_t kvHead, uint32_t r, uint32_t dim, const float4 &x) {
+    const uint32_t tok = token0 + r / p.group, head = kvHead * p.group + r % p.group;
+    const size_t at = (static_cast<size_t>(tok) * p.nHeads + head) * hd + dim;
+    if (p.half) *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + at) = make_uint2(packHalf2(x.x, x.y), packHalf2(x.z, x.w));
+    else *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = x;
+}
+
+// The producer warp of the kernels whose consumers share a tile's rows (paged_attn.cu, paged_steps.cu): hands on the items of the block's run
+// and requests their tiles into the ring, K and V and an int8 store's scales.  L: the kernel's layout.
+template <typename L>
+__device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUtensorMap &tmK, const CUtensorMap &tmV, uint8_t *smem, uint64_t *full,
+                                             uint64_t *empty, uint64_t *itemFull, PaItem *items) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t g = 0;  // tiles so far
+                    const uint32_t boxes = kPaTile / p.box, boxBytes = p.box * 128u;
+            if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
+            PagedWalk w;
+            uint32_t handed = 0;  // items
+            bool ok = true;
+            if (w.begin(p, L::MR, 0u, 1u)) do {
+                const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
+                const uint32_t t1 = w.last();
+                if (lane == 0) {
+                    PaItem it;
+                    it.t0 = w.first(), it.nTiles = t1 - it.t0, it.m0 = w.item * L::MR, it.rows = w.s.rows, it.token0 = w.s.token0;
+                    it.kvHead = w.kvHead, it.len = w.s.len, it.before = w.s.before;
+                    it.whole = it.t0 == 0u && t1 == w.tiles, it.part = 0;
+                    if (!it.whole) {
+                        const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
+                        it.part = blockIdx.x == c0 ? 1u : 0u;
+                        if (it.part) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
+                    }
+                    items[handed % kPaItems] = it;
+                    mbarArrive(&itemFull[handed % kPaItems]);
+                }
+                ++handed;
+                // where this lane's box of a tile lies: looked up a tile ahead
+                struct At {
+                    uint32_t have, in;
+                    int32_t page;
+                };
+                auto look = [&](uint32_t t) {
+                    const uint32_t row0 = t * kPaTile;
+                    At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
+                    if (lane < at.have) {
+                        const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
+                        at.in = row - slot * p.c.pageRows;
+                        at.page = __ldg(table + slot);
+                    }
+                    return at;
+                };
+                At next = look(w.first());
+                for (uint32_t t = w.first(); t < t1; ++t, ++g) {
+                    const uint32_t n = next.have, in = next.in;
+                    uint32_t page = static_cast<uint32_t>(next.page);
+                    next = look(t + 1u);
+                    if (lane < n && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
+                        atomicOr(p.c.err, kDevErrRowBound);
+                        page = 0;
+                    }
+                    const uint32_t st = g % uint32_t(L::NST);
+                    if (g >= uint32_t(L::NST)) ok = pfWait<true>(&empty[st], ((g / uint32_t(L::NST)) - 1u) & 1u, p.c.err, kDevErrEmptyWait);
+                    if (!ok) break;
+                    if (lane == 0) mbarExpectTx(&full[st], n * boxBytes * 2u * L::kPanels);
+                    __syncwarp();
+                    uint8_t *stage = smem + st * L::kStage;
+                    if (lane < n) {
+    #pragma unroll
+                        for (int h = 0; h < L::kPanels; ++h) {
+                            tmaLoad4D(stage + h * L::kPanel + lane * boxBytes, &tmK, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
+                            tmaLoad4D(stage + L::kMat + h * L::kPanel + lane * boxBytes, &tmV, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
+                        }
+                    }
+                    if constexpr (L::kI8) {
+                        float *sc = reinterpret_cast<float *>(smem + L::kScales) + st * 128u;
+    #pragma unroll
+                        for (uint32_t u = 0; u < 2; ++u) {
+                            const uint32_t key = lane + 32u * u, from = key / p.box;
+                            const uint32_t pg = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, in, from) + key - from * p.box;
+                            if (from < n) {
+                                const size_t at = (static_cast<size_t>(pg) * p.c.pageRows + r) * p.c.nKV + w.kvHead;
+                                cpAsync4(sc + key, p.ks + at);
+                                cpAsync4(sc + 64u + key, p.vs + at);
+                            }
+                        }
+                        cpAsyncMbarArriveNoinc(&full[st]);
+                    }
+                }
+            } while (ok && w.next(p));
+            if (lane == 0) {
+                items[handed % kPaItems].nTiles = 0u;
+                mbarArrive(&itemFull[handed % kPaItems]);
+            }
+            // no copy is under way any more when the block leaves
+            for (uint32_t back = 1; back <= uint32_t(L::NST) && back <= g; ++back)
+                if (!pfWait<true>(&full[(g - back) % uint32_t(L::NST)], ((g - back) / uint32_t(L::NST)) & 1u, p.c.err, kDevErrFullWait)) break;
+}
 #endif
 
 // paged_tiles.cu: the sequences of minRows query rows per kv head and more, fp16 queries, on tcgen05
 int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st);
 constexpr int kPagedSMs = 148;      // blocks that the workspace has room for, per block of an SM
 constexpr uint32_t kPagedTile = 128;  // query rows of a tile of the tiles kernel
+
+// The workspace: two partials per block of the two kernels' widest grids, then what the merge finds per block.
+constexpr size_t kRowsParts = size_t(2) * kPagedSMs * 2 * pagedSlot(64, 128);       // f32
+constexpr size_t kTilesParts = size_t(2) * kPagedSMs * pagedSlot(2 * kPagedTile, 128);
+static_assert(2 * pagedSlot(64, 128) >= pagedSlot(64, 256) && pagedSlot(2 * kPagedTile, 128) >= pagedSlot(kPagedTile, 256), "one block per SM at head_dim 256");
+constexpr size_t kPagedWorkspace = (kRowsParts + kTilesParts) * 4 + size_t(kPagedSMs) * 4 * sizeof(PagedJoin) + 32;
+
+// paged_steps.cu: up to pagedStepRows query rows per kv head; *blocks: its grid
+uint32_t pagedStepRows(const tc_paged_kv *c);
+int pagedAttnSteps(const tc_paged_kv *c, const PagedAttnParams &p, uint32_t rows, cudaStream_t st, uint32_t *blocks);
 
 int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v);  // maps of the pools, `box` rows a copy
 
