@@ -181,8 +181,6 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         tmaPrefetchDesc(&tmV);
     }
     __syncthreads();
-    gridDepWait();
-    gridDepLaunch();
     uint32_t g = 0;  // tiles so far
     if constexpr (L::kSplitRegs) {
         if (warp >= L::NW) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -195,6 +193,8 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         return;
     }
 
+    gridDepWait();
+    gridDepLaunch();
     // --------------------------------- consumers ---------------------------------
     const uint32_t wm = warp / WK, wk = warp % WK, c = lane & 3u, n8 = lane >> 2;
     constexpr int NR = PAIR ? 1 : 2;      // query rows of a thread: n8 (and n8 + 8)
@@ -550,6 +550,7 @@ int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v
     key.strides[2] = key.strides[1] * c->pageRows;
     key.box[0] = 128 / e, key.box[1] = 1, key.box[2] = box, key.box[3] = 1;
     key.rank = 4, key.elemBytes = e, key.swizzle = 3;
+    key.promote128 = c->hd * e == 128;  // (256 would bring a row of the next kv head, which another block asks for much later)
     key.base = c->k;
     const int rc = getTensorMap(key, k);
     if (rc != TC_OK) return rc;

@@ -106,26 +106,34 @@ struct PagedSeq {
     __device__ __forceinline__ uint64_t tilesAll(uint32_t MR, uint32_t group) const { return rows == 0u ? 0u : tilesBefore(MR, items(MR), group); }
 };
 
-__device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, uint32_t b) {
-    const uint32_t s0 = seqStart(p.c, b), s1 = min(seqStart(p.c, b + 1u), p.c.tokens);
+// What the tables say of a sequence.  Read through L2: a block may look before the kernels ahead of it are complete (PagedWalk::prepare).
+struct PagedRaw {
+    uint32_t start, stop, len;
+    __device__ __forceinline__ bool operator==(const PagedRaw &o) const { return start == o.start && stop == o.stop && len == o.len; }
+};
+__device__ __forceinline__ PagedRaw pagedRaw(const PagedAttnParams &p, uint32_t b) {
+    PagedRaw r;
+    if (p.c.starts != nullptr) r.start = __ldcg(p.c.starts + b), r.stop = __ldcg(p.c.starts + b + 1u);
+    else r.start = b * p.c.perSeq, r.stop = r.start + p.c.perSeq;
+    r.len = __ldcg(p.c.lens + b);
+    return r;
+}
+__device__ __forceinline__ uint32_t pagedMost(const PagedAttnParams &p) { return p.c.pagesPerSeq * p.c.pageRows; }  // rows that a sequence has pages for
+__device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, const PagedRaw &r) {
+    const uint32_t stop = min(r.stop, p.c.tokens), n = stop > r.start ? stop - r.start : 0u;
     PagedSeq s;
-    const uint32_t n = s1 > s0 ? s1 - s0 : 0u, most = p.c.pagesPerSeq * p.c.pageRows;
-    uint32_t len = __ldg(p.c.lens + b);
-    if (len > most) {  // more rows than the table has pages for
-        atomicOr(p.c.err, kDevErrRowBound);
-        len = most;
-    }
     s.rows = n * p.group;
     if (s.rows < p.minRows || s.rows > p.maxRows) s.rows = 0u;
-    s.len = len;
-    s.before = static_cast<int32_t>(len) - static_cast<int32_t>(n);
-    s.token0 = s0;
+    s.len = min(r.len, pagedMost(p));
+    s.before = static_cast<int32_t>(s.len) - static_cast<int32_t>(n);
+    s.token0 = r.start;
     return s;
 }
 
 // A walk over a block's run of units, item by item; every warp makes its own, in step.
 struct PagedWalk {
     uint32_t mr, over;        // query rows of an item; units ahead of its tiles that stand for what an item costs beside them
+    PagedRaw raw;             // sequence `lane`
     uint64_t total, at, end;  // units of the launch; the block's next and last
     uint32_t blocks;          // blocks with work
     uint32_t seq, kvHead, item;
@@ -139,19 +147,40 @@ struct PagedWalk {
     __device__ __forceinline__ uint64_t unitsAll(const PagedSeq &q, uint32_t group) const { return q.tilesAll(mr, group) + static_cast<uint64_t>(over) * q.items(mr); }
     __device__ __forceinline__ uint64_t unitsBefore(uint32_t m, uint32_t group) const { return s.tilesBefore(mr, m, group) + static_cast<uint64_t>(over) * m; }
 
-    // All lanes of the warp.  False: nothing to do.  leastRun: units that a block has at least, where there are so many.
-    __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead, uint32_t leastRun) {
+    // What begin() finds in its first look, before the kernels ahead in the stream are complete: the chain of loads and quotients at a
+    // block's start (4 us, most of it instructions that come from far) then passes under them.  As a rule the tables are older than
+    // those kernels; start() looks again and begins anew where they were not.
+    __device__ __forceinline__ bool prepare(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
+        const uint32_t lane = threadIdx.x & 31u;
+        raw = lane < p.c.batch ? pagedRaw(p, lane) : PagedRaw{0u, 0u, 0u};
+        return begin(p, itemRows, overhead);
+    }
+    // Behind the wait for those kernels.  some: what prepare() said.
+    __device__ __forceinline__ bool start(const PagedAttnParams &p, bool some) {
+        const uint32_t lane = threadIdx.x & 31u;
+        const PagedRaw now = lane < p.c.batch ? pagedRaw(p, lane) : PagedRaw{0u, 0u, 0u};
+        if (blockIdx.x == 0)
+            for (uint32_t b = lane; b < p.c.batch; b += 32u)
+                if (pagedRaw(p, b).len > pagedMost(p)) atomicOr(p.c.err, kDevErrRowBound);  // more rows than the table has pages for
+        const bool same = p.c.batch <= 32u && now == raw;
+        if (__all_sync(0xffffffffu, same)) return some;
+        raw = now;
+        return begin(p, mr, over);
+    }
+
+    // All lanes of the warp.  False: nothing to do.
+    __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
         mr = itemRows, over = overhead;
         const uint32_t lane = threadIdx.x & 31u;
-        auto unitsOf = [&](uint32_t b) { return b < p.c.batch ? unitsAll(pagedSeq(p, b), p.group) * p.c.nKV : 0u; };
-        const uint64_t lead = unitsOf(lane);  // of the first 32 sequences
+        auto unitsOf = [&](uint32_t b) { return b < p.c.batch ? unitsAll(pagedSeq(p, pagedRaw(p, b)), p.group) * p.c.nKV : 0u; };
+        const uint64_t lead = lane < p.c.batch ? unitsAll(pagedSeq(p, raw), p.group) * p.c.nKV : 0u;  // of the first 32 sequences
         uint64_t sum = lead;
         for (uint32_t b0 = 32u; b0 < p.c.batch; b0 += 32u) sum += unitsOf(b0 + lane);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum;
         if (total == 0u) return false;
-        blocks = static_cast<uint32_t>(max(static_cast<uint64_t>(1), min(static_cast<uint64_t>(gridDim.x), divide(total, leastRun))));
+        blocks = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x), total));
         if (blockIdx.x >= blocks) return false;
         at = firstOf(blockIdx.x), end = firstOf(blockIdx.x + 1u);
         // the sequence that holds unit `at`
@@ -174,7 +203,11 @@ struct PagedWalk {
             base += __shfl_sync(0xffffffffu, upTo, 31);
             if (b0 + 32u >= p.c.batch) return false;  // (not reached: `at` lies below the sum)
         }
-        s = pagedSeq(p, seq);
+        // (out of the registers that found it: what the tables say may change until start())
+        PagedRaw found{__shfl_sync(0xffffffffu, raw.start, seq & 31u), __shfl_sync(0xffffffffu, raw.stop, seq & 31u), __shfl_sync(0xffffffffu, raw.len, seq & 31u)};
+        if (seq >= 32u) found = pagedRaw(p, seq);
+        s = pagedSeq(p, found);
+        if (s.rows == 0u) return false;  // (only where the tables changed meanwhile)
         uint64_t in = at - base;
         kvHead = 0;
         if (p.c.nKV > 1u) {
@@ -211,7 +244,7 @@ struct PagedWalk {
                 kvHead = 0;
                 do {
                     if (++seq >= p.c.batch) return false;  // (not reached: the run is not done)
-                    s = pagedSeq(p, seq);
+                    s = pagedSeq(p, pagedRaw(p, seq));
                 } while (s.rows == 0u);
             }
         }
@@ -262,88 +295,91 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
                                              uint64_t *empty, uint64_t *itemFull, PaItem *items) {
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t g = 0;  // tiles so far
-                    const uint32_t boxes = kPaTile / p.box, boxBytes = p.box * 128u;
-            if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
-            PagedWalk w;
-            uint32_t handed = 0;  // items
-            bool ok = true;
-            if (w.begin(p, L::MR, 0u, 1u)) do {
-                const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
-                const uint32_t t1 = w.last();
-                if (lane == 0) {
-                    PaItem it;
-                    it.t0 = w.first(), it.nTiles = t1 - it.t0, it.m0 = w.item * L::MR, it.rows = w.s.rows, it.token0 = w.s.token0;
-                    it.kvHead = w.kvHead, it.len = w.s.len, it.before = w.s.before;
-                    it.whole = it.t0 == 0u && t1 == w.tiles, it.part = 0;
-                    if (!it.whole) {
-                        const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
-                        it.part = blockIdx.x == c0 ? 1u : 0u;
-                        if (it.part) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
-                    }
-                    items[handed % kPaItems] = it;
-                    mbarArrive(&itemFull[handed % kPaItems]);
-                }
-                ++handed;
-                // where this lane's box of a tile lies: looked up a tile ahead
-                struct At {
-                    uint32_t have, in;
-                    int32_t page;
-                };
-                auto look = [&](uint32_t t) {
-                    const uint32_t row0 = t * kPaTile;
-                    At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
-                    if (lane < at.have) {
-                        const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
-                        at.in = row - slot * p.c.pageRows;
-                        at.page = __ldg(table + slot);
-                    }
-                    return at;
-                };
-                At next = look(w.first());
-                for (uint32_t t = w.first(); t < t1; ++t, ++g) {
-                    const uint32_t n = next.have, in = next.in;
-                    uint32_t page = static_cast<uint32_t>(next.page);
-                    next = look(t + 1u);
-                    if (lane < n && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
-                        atomicOr(p.c.err, kDevErrRowBound);
-                        page = 0;
-                    }
-                    const uint32_t st = g % uint32_t(L::NST);
-                    if (g >= uint32_t(L::NST)) ok = pfWait<true>(&empty[st], ((g / uint32_t(L::NST)) - 1u) & 1u, p.c.err, kDevErrEmptyWait);
-                    if (!ok) break;
-                    if (lane == 0) mbarExpectTx(&full[st], n * boxBytes * 2u * L::kPanels);
-                    __syncwarp();
-                    uint8_t *stage = smem + st * L::kStage;
-                    if (lane < n) {
-    #pragma unroll
-                        for (int h = 0; h < L::kPanels; ++h) {
-                            tmaLoad4D(stage + h * L::kPanel + lane * boxBytes, &tmK, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
-                            tmaLoad4D(stage + L::kMat + h * L::kPanel + lane * boxBytes, &tmV, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
-                        }
-                    }
-                    if constexpr (L::kI8) {
-                        float *sc = reinterpret_cast<float *>(smem + L::kScales) + st * 128u;
-    #pragma unroll
-                        for (uint32_t u = 0; u < 2; ++u) {
-                            const uint32_t key = lane + 32u * u, from = key / p.box;
-                            const uint32_t pg = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, in, from) + key - from * p.box;
-                            if (from < n) {
-                                const size_t at = (static_cast<size_t>(pg) * p.c.pageRows + r) * p.c.nKV + w.kvHead;
-                                cpAsync4(sc + key, p.ks + at);
-                                cpAsync4(sc + 64u + key, p.vs + at);
-                            }
-                        }
-                        cpAsyncMbarArriveNoinc(&full[st]);
-                    }
-                }
-            } while (ok && w.next(p));
-            if (lane == 0) {
-                items[handed % kPaItems].nTiles = 0u;
-                mbarArrive(&itemFull[handed % kPaItems]);
+    const uint32_t boxes = kPaTile / p.box, boxBytes = p.box * 128u;
+    PagedWalk w;
+    uint32_t handed = 0;  // items
+    bool ok = true;
+    const bool some = w.prepare(p, L::MR, 0u);
+    gridDepWait();
+    gridDepLaunch();
+    if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
+    if (w.start(p, some)) do {
+        const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
+        const uint32_t t1 = w.last();
+        if (lane == 0) {
+            PaItem it;
+            it.t0 = w.first(), it.nTiles = t1 - it.t0, it.m0 = w.item * L::MR, it.rows = w.s.rows, it.token0 = w.s.token0;
+            it.kvHead = w.kvHead, it.len = w.s.len, it.before = w.s.before;
+            it.whole = it.t0 == 0u && t1 == w.tiles, it.part = 0;
+            if (!it.whole) {
+                const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
+                it.part = blockIdx.x == c0 ? 1u : 0u;
+                if (it.part) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
             }
-            // no copy is under way any more when the block leaves
-            for (uint32_t back = 1; back <= uint32_t(L::NST) && back <= g; ++back)
-                if (!pfWait<true>(&full[(g - back) % uint32_t(L::NST)], ((g - back) / uint32_t(L::NST)) & 1u, p.c.err, kDevErrFullWait)) break;
+            items[handed % kPaItems] = it;
+            mbarArrive(&itemFull[handed % kPaItems]);
+        }
+        ++handed;
+        // where this lane's box of a tile lies: looked up a tile ahead
+        struct At {
+            uint32_t have, in;
+            int32_t page;
+        };
+        auto look = [&](uint32_t t) {
+            const uint32_t row0 = t * kPaTile;
+            At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
+            if (lane < at.have) {
+                const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
+                at.in = row - slot * p.c.pageRows;
+                at.page = __ldg(table + slot);
+            }
+            return at;
+        };
+        At next = look(w.first());
+        for (uint32_t t = w.first(); t < t1; ++t, ++g) {
+            const uint32_t n = next.have, in = next.in;
+            uint32_t page = static_cast<uint32_t>(next.page);
+            next = look(t + 1u);
+            if (lane < n && page >= p.c.numPages) {  // no such page: reported, page 0 stands in
+                atomicOr(p.c.err, kDevErrRowBound);
+                page = 0;
+            }
+            const uint32_t st = g % uint32_t(L::NST);
+            if (g >= uint32_t(L::NST)) ok = pfWait<true>(&empty[st], ((g / uint32_t(L::NST)) - 1u) & 1u, p.c.err, kDevErrEmptyWait);
+            if (!ok) break;
+            if (lane == 0) mbarExpectTx(&full[st], n * boxBytes * 2u * L::kPanels);
+            __syncwarp();
+            uint8_t *stage = smem + st * L::kStage;
+            if (lane < n) {
+    #pragma unroll
+                for (int h = 0; h < L::kPanels; ++h) {
+                    tmaLoad4D(stage + h * L::kPanel + lane * boxBytes, &tmK, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
+                    tmaLoad4D(stage + L::kMat + h * L::kPanel + lane * boxBytes, &tmV, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
+                }
+            }
+            if constexpr (L::kI8) {
+                float *sc = reinterpret_cast<float *>(smem + L::kScales) + st * 128u;
+    #pragma unroll
+                for (uint32_t u = 0; u < 2; ++u) {
+                    const uint32_t key = lane + 32u * u, from = key / p.box;
+                    const uint32_t pg = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, in, from) + key - from * p.box;
+                    if (from < n) {
+                        const size_t at = (static_cast<size_t>(pg) * p.c.pageRows + r) * p.c.nKV + w.kvHead;
+                        cpAsync4(sc + key, p.ks + at);
+                        cpAsync4(sc + 64u + key, p.vs + at);
+                    }
+                }
+                cpAsyncMbarArriveNoinc(&full[st]);
+            }
+        }
+    } while (ok && w.next(p));
+    if (lane == 0) {
+        items[handed % kPaItems].nTiles = 0u;
+        mbarArrive(&itemFull[handed % kPaItems]);
+    }
+    // no copy is under way any more when the block leaves
+    for (uint32_t back = 1; back <= uint32_t(L::NST) && back <= g; ++back)
+        if (!pfWait<true>(&full[(g - back) % uint32_t(L::NST)], ((g - back) / uint32_t(L::NST)) & 1u, p.c.err, kDevErrFullWait)) break;
 }
 #endif
 

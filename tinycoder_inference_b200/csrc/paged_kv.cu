@@ -6,6 +6,7 @@
 // Both stream: HBM bounds the prompts, the chain starts -> lens -> page -> row the single tokens, so the rows that do
 // not depend on it are requested ahead of it.
 #include "paged.cuh"
+#include "tc_tcgen05.cuh"
 
 namespace tc {
 
@@ -151,14 +152,48 @@ struct PagedReadParams {
     const void *kc, *vc;
     const float *ks, *vs;
     void *kOut, *vOut;
-    uint32_t unitsPerToken;
+    uint32_t unitsPerToken, out32;  // out32: the outputs are 32-byte aligned
 };
 
-// A lane takes 16 bytes of a store row (16 int8 or 8 fp16 values), a group of lanes the row; a group takes U rows of one token (the kv
-// heads of K, then those of V).
-template <int HD, bool I8, bool HALF, int U>
+// 16 bytes of a store row as f32 or fp16 values from element `at` on
+template <bool I8, bool HALF>
+__device__ __forceinline__ void pagedPut(void *out, size_t at, const uint4 &raw, float sc, bool out32) {
+    constexpr uint32_t E = I8 ? 16 : 8;
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (!I8 && HALF) {
+        *reinterpret_cast<uint4 *>(static_cast<__half *>(out) + at) = raw;
+    } else {
+        float f[E];
+#pragma unroll
+        for (uint32_t e = 0; e < E; ++e) {
+            if constexpr (I8) f[e] = static_cast<float>(static_cast<int8_t>((w[e / 4] >> (8 * (e % 4))) & 0xffu)) * sc;
+            else f[e] = __half2float(__ushort_as_half(static_cast<unsigned short>((w[e / 2] >> (16 * (e % 2))) & 0xffffu)));
+        }
+        constexpr uint32_t N = HALF ? E / 2 : E;  // words
+        uint32_t o[N];
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) o[i] = HALF ? packHalf2(f[2 * i], f[2 * i + (HALF ? 1 : 0)]) : __float_as_uint(f[i]);
+        uint32_t *d = HALF ? reinterpret_cast<uint32_t *>(static_cast<__half *>(out) + at) : reinterpret_cast<uint32_t *>(static_cast<float *>(out) + at);
+        // 32 bytes a store, whole sectors: 16 bytes at a stride of 32 take 46 us for what these take 36 (60000 int8 rows of 4 x 128 to fp16)
+#pragma unroll
+        for (uint32_t i = 0; i < N; i += 8) {
+            if (N >= 8 && out32) {
+                stGlobalV8(reinterpret_cast<float *>(d + i), __uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]),
+                           __uint_as_float(o[i + (N >= 8 ? 4 : 0)]), __uint_as_float(o[i + (N >= 8 ? 5 : 1)]), __uint_as_float(o[i + (N >= 8 ? 6 : 2)]),
+                           __uint_as_float(o[i + (N >= 8 ? 7 : 3)]));
+            } else {
+#pragma unroll
+                for (uint32_t k = i; k < i + 8 && k < N; k += 4) *reinterpret_cast<uint4 *>(d + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            }
+        }
+    }
+}
+
+// A lane takes 16 bytes of a store row (16 int8 or 8 fp16 values), a group of lanes the row.  For few rows, where the chain
+// starts -> lens -> page -> row is all there is.
+template <int HD, bool I8, bool HALF>
 __global__ void __launch_bounds__(256) pagedReadKernel(const __grid_constant__ PagedReadParams p) {
-    constexpr uint32_t E = I8 ? 16 : 8, G = HD / E;  // values of a lane; lanes of a row
+    constexpr uint32_t E = I8 ? 16 : 8, G = HD / E, U = 1;  // values of a lane; lanes of a row; rows of a group
     const uint32_t unit = blockIdx.x * (256u / G) + threadIdx.x / G;
     const uint32_t i = threadIdx.x & (G - 1u);
     const uint32_t t = unit / p.unitsPerToken, first = (unit - t * p.unitsPerToken) * U;
@@ -191,26 +226,68 @@ __global__ void __launch_bounds__(256) pagedReadKernel(const __grid_constant__ P
         const bool isV = r >= p.c.nKV;
         const size_t at = ((static_cast<size_t>(t) * p.c.nKV + (isV ? r - p.c.nKV : r)) * G + i) * E;
         void *out = isV ? p.vOut : p.kOut;
-        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-        if constexpr (!I8 && HALF) {
-            *reinterpret_cast<uint4 *>(static_cast<__half *>(out) + at) = raw[u];
-        } else {
-            float f[E];
-#pragma unroll
-            for (uint32_t e = 0; e < E; ++e) {
-                if constexpr (I8) f[e] = static_cast<float>(static_cast<int8_t>((w[e / 4] >> (8 * (e % 4))) & 0xffu)) * sc[u];
-                else f[e] = __half2float(__ushort_as_half(static_cast<unsigned short>((w[e / 2] >> (16 * (e % 2))) & 0xffffu)));
-            }
-            if constexpr (HALF) {
-#pragma unroll
-                for (uint32_t e = 0; e < E; e += 8)
-                    *reinterpret_cast<uint4 *>(static_cast<__half *>(out) + at + e) =
-                            make_uint4(packHalf2(f[e], f[e + 1]), packHalf2(f[e + 2], f[e + 3]), packHalf2(f[e + 4], f[e + 5]), packHalf2(f[e + 6], f[e + 7]));
+        pagedPut<I8, HALF>(out, at, raw[u], sc[u], p.out32 != 0u);
+    }
+}
+
+// The same for many rows: a block takes kReadTokens tokens.  One warp looks them up, a lane each, and leaves their rows in shared memory; then
+// every thread has U loads under way that wait for nothing else.  (A group of lanes that looks its own token up every four rows spends
+// more than half of its time on that chain: 60000 rows of 4 x 128 int8 to fp16 43 us.)
+constexpr uint32_t kReadTokens = 32;
+template <int HD, bool I8, bool HALF>
+__global__ void __launch_bounds__(256) pagedReadManyKernel(const __grid_constant__ PagedReadParams p) {
+    constexpr uint32_t E = I8 ? 16 : 8, G = HD / E, U = 4;
+    __shared__ int64_t rowS[kReadTokens];  // -1: no page; -2: behind the last sequence
+    gridDepWait();
+    gridDepLaunch();
+    const uint32_t t0 = blockIdx.x * kReadTokens;
+    if (threadIdx.x < kReadTokens) {
+        const uint32_t t = t0 + threadIdx.x;
+        int64_t at = -2;
+        if (t < p.c.tokens) {
+            uint32_t b = 0, n = p.c.batch, end;
+            if (p.c.starts == nullptr) {
+                b = t / p.c.perSeq, end = (b + 1u) * p.c.perSeq;
             } else {
-#pragma unroll
-                for (uint32_t e = 0; e < E; e += 4)
-                    *reinterpret_cast<float4 *>(static_cast<float *>(out) + at + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                while (n > 1u) {  // the last sequence that does not start behind t
+                    const uint32_t half = n / 2u;
+                    const bool right = __ldg(p.c.starts + b + half) <= t;
+                    b += right ? half : 0u, n = right ? n - half : half;
+                }
+                end = __ldg(p.c.starts + b + 1u);
             }
+            if (t < end) {
+                size_t row;
+                at = pagedRow(p.c, b, static_cast<int64_t>(__ldg(p.c.lens + b)) - static_cast<int64_t>(end - t), row) ? static_cast<int64_t>(row) : -1;
+                if (at < 0) atomicOr(p.c.err, kDevErrRowBound);
+            }
+        }
+        rowS[threadIdx.x] = at;
+    }
+    __syncthreads();
+    const uint32_t perToken = 2u * p.c.nKV * G, units = min(kReadTokens, p.c.tokens - t0) * perToken;
+    for (uint32_t u0 = threadIdx.x; u0 < units; u0 += U * 256u) {
+        uint4 raw[U];
+        float sc[U];
+        uint32_t tok[U], rest[U];
+#pragma unroll
+        for (uint32_t k = 0; k < U; ++k) {
+            const uint32_t u = u0 + k * 256u;
+            raw[k] = make_uint4(0u, 0u, 0u, 0u), sc[k] = 0.0f;
+            tok[k] = u / perToken, rest[k] = u - tok[k] * perToken;
+            if (u >= units) continue;
+            const int64_t row = rowS[tok[k]];
+            if (row < 0) continue;
+            const uint32_t r = rest[k] / G, head = r >= p.c.nKV ? r - p.c.nKV : r;
+            const size_t rowHead = static_cast<size_t>(row) * p.c.nKV + head;
+            raw[k] = __ldg(static_cast<const uint4 *>(r >= p.c.nKV ? p.vc : p.kc) + rowHead * G + rest[k] % G);
+            if (I8) sc[k] = __ldg((r >= p.c.nKV ? p.vs : p.ks) + rowHead);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < U; ++k) {
+            if (u0 + k * 256u >= units || rowS[tok[k]] == -2) continue;
+            const uint32_t r = rest[k] / G, head = r >= p.c.nKV ? r - p.c.nKV : r;
+            pagedPut<I8, HALF>(r >= p.c.nKV ? p.vOut : p.kOut, ((static_cast<size_t>(t0 + tok[k]) * p.c.nKV + head) * G + rest[k] % G) * E, raw[k], sc[k], p.out32 != 0u);
         }
     }
 }
@@ -275,18 +352,19 @@ int tc_paged_kv_read(const tc_paged_kv *c, void *kOut, void *vOut, int outHalf, 
     TC_REQUIRE(((reinterpret_cast<uintptr_t>(kOut) | reinterpret_cast<uintptr_t>(vOut)) & 15u) == 0, TC_EINVAL, "paged read: alignment (16 bytes)");
     unsigned int *err = devErrorWord();
     TC_REQUIRE(err != nullptr, TC_ECUDA, "no CUDA device");
-    PagedReadParams p{pagedView(c, err), c->k, c->v, c->ks, c->vs, kOut, vOut, 0};
+    PagedReadParams p{pagedView(c, err), c->k, c->v, c->ks, c->vs, kOut, vOut, 0, 0};
+    p.out32 = ((reinterpret_cast<uintptr_t>(kOut) | reinterpret_cast<uintptr_t>(vOut)) & 31u) == 0;
     const uint32_t rows = 2 * c->nKV, lanes = c->hd / (c->kvI8 ? 16 : 8);
     const bool many = manyRows(static_cast<uint64_t>(c->tokens) * rows, lanes);
-    p.unitsPerToken = many ? (rows + kManyRows - 1) / kManyRows : rows;
+    p.unitsPerToken = rows;
     uint32_t blocks;
-    const int gc = pagedGrid(static_cast<uint64_t>(c->tokens) * p.unitsPerToken, lanes, &blocks);
+    const int gc = pagedGrid(static_cast<uint64_t>(c->tokens) * rows, lanes, &blocks);
     if (gc != TC_OK) return gc;
-    auto pick = [&](auto half1, auto half4, auto f1, auto f4) {
-        return launchDependent(outHalf ? (many ? half4 : half1) : (many ? f4 : f1), dim3(blocks), 256, 0, static_cast<cudaStream_t>(stream), 1, p);
-    };
+    if (many) blocks = (c->tokens + kReadTokens - 1) / kReadTokens;
+    auto go = [&](auto kern) { return launchDependent(kern, dim3(blocks), 256, 0, static_cast<cudaStream_t>(stream), 1, p); };
 #define TC_PAGED_READ(HD, I8) \
-    pick(pagedReadKernel<HD, I8, true, 1>, pagedReadKernel<HD, I8, true, kManyRows>, pagedReadKernel<HD, I8, false, 1>, pagedReadKernel<HD, I8, false, kManyRows>)
+    (many ? (outHalf ? go(pagedReadManyKernel<HD, I8, true>) : go(pagedReadManyKernel<HD, I8, false>)) \
+          : (outHalf ? go(pagedReadKernel<HD, I8, true>) : go(pagedReadKernel<HD, I8, false>)))
     if (c->kvI8) return c->hd == 128 ? TC_PAGED_READ(128, true) : TC_PAGED_READ(256, true);
     if (c->hd == 64) return TC_PAGED_READ(64, false);
     return c->hd == 128 ? TC_PAGED_READ(128, false) : TC_PAGED_READ(256, false);

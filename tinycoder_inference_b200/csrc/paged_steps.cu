@@ -61,12 +61,13 @@ pagedStepsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         tmaPrefetchDesc(&tmV);
     }
     __syncthreads();
-    gridDepWait();
-    gridDepLaunch();
     if (warp == L::NW) {
         pagedProduce<L>(p, tmK, tmV, smem, full, empty, itemFull, items);
         return;
     }
+
+    gridDepWait();
+    gridDepLaunch();
 
     const uint32_t c = lane & 3u, n8 = lane >> 2, key0 = warp * 16u;
     constexpr int NS = L::NS, NM = HD / 16, QW = EXACT ? 4 : 2;  // steps of q . K; 16-dim output tiles; registers of a step's q

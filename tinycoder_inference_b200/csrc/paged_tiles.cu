@@ -22,13 +22,8 @@ namespace tc {
 
 constexpr int kPtScales = 132;          // f32 of a scale slot: K's 64, V's 64, the power of two above V's; padding
 constexpr uint32_t kPtScaleSlots = 16;
-#ifndef PT_OVER
-#define PT_OVER 2
-#endif
-#ifndef PT_RUN
-#define PT_RUN 1
-#endif
-constexpr uint32_t kPtOver = PT_OVER, kPtRun = PT_RUN;
+// What an item costs beside its tiles, in tiles: four whole prompts take 371 us with 0, 340 with 2, 347 with 3 and 358 with 6.
+constexpr uint32_t kPtOver = 2;
 constexpr int kPtBN = int(kPaTile);
 constexpr float kPtLazyLog2 = 8.0f;  // O is rescaled when the row's maximum ran ahead by 2^8
 constexpr float kPtOff = 6.0f;       // probabilities are held as 2^6 p, at most 2^14: what fp16 has above them goes to the small ones
@@ -164,9 +159,11 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     __syncthreads();
     tcFenceAfter();
     const uint32_t tmemBase = *reinterpret_cast<volatile uint32_t *>(tmemSlot);
-    gridDepWait();
-    gridDepLaunch();
     const uint32_t tileRows = p.tileTokens * p.group;
+    if (warp != 8) {
+        gridDepWait();
+        gridDepLaunch();
+    }
     // The n-th item of the block, once the producer has put it down; false: there is none any more.
     auto takeItem = [&](uint32_t n, const PtItem *&it) {
         it = &items[n % kPtItems];
@@ -243,11 +240,13 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (warp == 8) {
         // ------------------------------- producer -------------------------------
         uint32_t gk = 0, gs = 0, n = 0;
-        if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
         PagedWalk w;
-        const bool some = w.begin(p, tileRows * L::kQTiles, kPtOver, kPtRun);
+        const bool some = w.prepare(p, tileRows * L::kQTiles, kPtOver);
+        gridDepWait();
+        gridDepLaunch();
+        if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
         bool ok = true;
-        if (some) do {
+        if (w.start(p, some)) do {
             uint32_t joins;
             const PtItem it = ptItem<kOne>(p, w, joins);
             if (lane == 0) {

@@ -55,7 +55,7 @@ struct TensorMapKey {
     uint64_t strides[3];  // bytes, dims 1..3
     uint32_t box[4];
     uint32_t rank, elemBytes, swizzle;  // swizzle: 0 none, 1 32B, 2 64B, 3 128B
-    uint32_t pad_;                      // keeps the struct free of implicit padding (it is memcmp'd)
+    uint32_t promote128;                // 1: L2 takes 128 bytes of a miss, else 256 (the field also keeps the struct, which is memcmp'd, without padding)
 };
 int getTensorMap(const TensorMapKey &key, CUtensorMap *out);
 

@@ -140,7 +140,8 @@ int getTensorMap(const TensorMapKey &key, CUtensorMap *out) {
                                                : CU_TENSOR_MAP_SWIZZLE_NONE;
     CUtensorMap m;
     CUresult r = fn(&m, dt, key.rank, const_cast<void *>(key.base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                    key.promote128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     TC_REQUIRE(r == CUDA_SUCCESS, TC_ECUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int) r);
     {
