@@ -133,7 +133,8 @@ __device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, const Pag
 // A walk over a block's run of units, item by item; every warp makes its own, in step.
 struct PagedWalk {
     uint32_t mr, over;        // query rows of an item; units ahead of its tiles that stand for what an item costs beside them
-    PagedRaw raw;             // sequence `lane`
+    static constexpr uint32_t kHeld = 4;
+    PagedRaw raw[kHeld];      // sequences lane, 32 + lane, ..
     uint64_t total, at, end;  // units of the launch; the block's next and last
     uint32_t blocks;          // blocks with work
     uint32_t seq, kvHead, item;
@@ -151,31 +152,37 @@ struct PagedWalk {
     // block's start (4 us, most of it instructions that come from far) then passes under them.  As a rule the tables are older than
     // those kernels; start() looks again and begins anew where they were not.
     __device__ __forceinline__ bool prepare(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
-        const uint32_t lane = threadIdx.x & 31u;
-        raw = lane < p.c.batch ? pagedRaw(p, lane) : PagedRaw{0u, 0u, 0u};
+        look(p, raw);
         return begin(p, itemRows, overhead);
     }
     // Behind the wait for those kernels.  some: what prepare() said.
     __device__ __forceinline__ bool start(const PagedAttnParams &p, bool some) {
+        PagedRaw now[kHeld];
+        look(p, now);
         const uint32_t lane = threadIdx.x & 31u;
-        const PagedRaw now = lane < p.c.batch ? pagedRaw(p, lane) : PagedRaw{0u, 0u, 0u};
         if (blockIdx.x == 0)
             for (uint32_t b = lane; b < p.c.batch; b += 32u)
                 if (pagedRaw(p, b).len > pagedMost(p)) atomicOr(p.c.err, kDevErrRowBound);  // more rows than the table has pages for
-        const bool same = p.c.batch <= 32u && now == raw;
-        if (__all_sync(0xffffffffu, same)) return some;
-        raw = now;
-        return begin(p, mr, over);
+        bool same = p.c.batch <= 32u * kHeld;
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; ++k) same = same && now[k] == raw[k], raw[k] = now[k];
+        return __all_sync(0xffffffffu, same) ? some : begin(p, mr, over);
+    }
+    __device__ __forceinline__ void look(const PagedAttnParams &p, PagedRaw (&r)[kHeld]) const {
+        const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; ++k) r[k] = 32u * k + lane < p.c.batch ? pagedRaw(p, 32u * k + lane) : PagedRaw{0u, 0u, 0u};
     }
 
     // All lanes of the warp.  False: nothing to do.
     __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
         mr = itemRows, over = overhead;
         const uint32_t lane = threadIdx.x & 31u;
-        auto unitsOf = [&](uint32_t b) { return b < p.c.batch ? unitsAll(pagedSeq(p, pagedRaw(p, b)), p.group) * p.c.nKV : 0u; };
-        const uint64_t lead = lane < p.c.batch ? unitsAll(pagedSeq(p, raw), p.group) * p.c.nKV : 0u;  // of the first 32 sequences
-        uint64_t sum = lead;
-        for (uint32_t b0 = 32u; b0 < p.c.batch; b0 += 32u) sum += unitsOf(b0 + lane);
+        auto unitsOf = [&](uint32_t b, const PagedRaw &r) { return b < p.c.batch ? unitsAll(pagedSeq(p, r), p.group) * p.c.nKV : 0u; };
+        uint64_t held[kHeld], sum = 0;  // units of the first sequences, out of registers; the others are looked up
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; ++k) held[k] = unitsOf(32u * k + lane, raw[k]), sum += held[k];
+        for (uint32_t b = 32u * kHeld + lane; b < p.c.batch; b += 32u) sum += unitsOf(b, pagedRaw(p, b));
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum;
@@ -185,8 +192,9 @@ struct PagedWalk {
         at = firstOf(blockIdx.x), end = firstOf(blockIdx.x + 1u);
         // the sequence that holds unit `at`
         uint64_t base = 0;
-        for (uint32_t b0 = 0;; b0 += 32u) {
-            const uint64_t mine = b0 == 0u ? lead : unitsOf(b0 + lane);
+        bool have = false;
+        PagedRaw found{0u, 0u, 0u};
+        auto search = [&](uint32_t b0, uint64_t mine, const PagedRaw &r) {
             uint64_t upTo = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -194,18 +202,22 @@ struct PagedWalk {
                 if (lane >= static_cast<uint32_t>(o)) upTo += x;
             }
             const uint32_t past = __ballot_sync(0xffffffffu, base + upTo > at);
+            const int l = past != 0u ? __ffs(past) - 1 : 31;
             if (past != 0u) {
-                const int l = __ffs(past) - 1;
+                have = true;
                 seq = b0 + l;
-                base += __shfl_sync(0xffffffffu, upTo - mine, l);
-                break;
+                found.start = __shfl_sync(0xffffffffu, r.start, l), found.stop = __shfl_sync(0xffffffffu, r.stop, l), found.len = __shfl_sync(0xffffffffu, r.len, l);
             }
-            base += __shfl_sync(0xffffffffu, upTo, 31);
-            if (b0 + 32u >= p.c.batch) return false;  // (not reached: `at` lies below the sum)
+            base += __shfl_sync(0xffffffffu, past != 0u ? upTo - mine : upTo, l);
+        };
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; ++k)
+            if (!have && 32u * k < p.c.batch) search(32u * k, held[k], raw[k]);
+        for (uint32_t b0 = 32u * kHeld; !have && b0 < p.c.batch; b0 += 32u) {
+            const PagedRaw r = b0 + lane < p.c.batch ? pagedRaw(p, b0 + lane) : PagedRaw{0u, 0u, 0u};
+            search(b0, unitsOf(b0 + lane, r), r);
         }
-        // (out of the registers that found it: what the tables say may change until start())
-        PagedRaw found{__shfl_sync(0xffffffffu, raw.start, seq & 31u), __shfl_sync(0xffffffffu, raw.stop, seq & 31u), __shfl_sync(0xffffffffu, raw.len, seq & 31u)};
-        if (seq >= 32u) found = pagedRaw(p, seq);
+        if (!have) return false;  // (only where the tables changed meanwhile)
         s = pagedSeq(p, found);
         if (s.rows == 0u) return false;  // (only where the tables changed meanwhile)
         uint64_t in = at - base;
@@ -288,7 +300,42 @@ __device__ __forceinline__ void pagedStore(const PagedAttnParams &p, uint32_t hd
     else *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = x;
 }
 
-// The producer warp of the kernels whose consumers share a tile's rows (paged_attn.cu, paged_steps.cu): hands on the items of the block's run
+// A query row of f32 as fp16 pairs, four dims of it a step, dim(st) ..: put(st, {hi 0 1, hi 2 3, lo 0 1, lo 2 3}); the four lanes of a row work together.
+// The row's largest goes to [2^10, 2^11), so that what the upper half leaves is a normal fp16 number.  Returns what undoes that.
+template <int NS, typename D, typename P>
+__device__ __forceinline__ float pagedQuery(const PagedAttnParams &p, const PaItem &it, uint32_t rr, bool valid, uint32_t hd, D &&dim, P &&put) {
+    const uint32_t tok = it.token0 + rr / p.group, head = it.kvHead * p.group + rr % p.group;
+    const float *src = static_cast<const float *>(p.q) + (static_cast<size_t>(tok) * p.nHeads + head) * hd;
+    float4 x[NS];
+    float top = 0.0f;
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+        x[st] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (valid) x[st] = __ldg(reinterpret_cast<const float4 *>(src + dim(st)));
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[st].x), fabsf(x[st].y)), fmaxf(fabsf(x[st].z), fabsf(x[st].w))));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float up = 1.0f, back = 1.0f;
+    if (top > 0.0f && top < INFINITY) {
+        const int e = min(126, max(-116, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+        up = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
+        back = __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
+    }
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+        float h[4], l[4];
+        splitHalf(x[st].x * up, h[0], l[0]);
+        splitHalf(x[st].y * up, h[1], l[1]);
+        splitHalf(x[st].z * up, h[2], l[2]);
+        splitHalf(x[st].w * up, h[3], l[3]);
+        const uint32_t w[4] = {packHalf2(h[0], h[1]), packHalf2(h[2], h[3]), packHalf2(l[0], l[1]), packHalf2(l[2], l[3])};
+        put(st, w);
+    }
+    return back;
+}
+
+// The producer warp of the kernels whose consumers share a tile's rows (paged_rows.cu, paged_steps.cu): hands on the items of the block's run
 // and requests their tiles into the ring, K and V and an int8 store's scales.  L: the kernel's layout.
 template <typename L>
 __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUtensorMap &tmK, const CUtensorMap &tmV, uint8_t *smem, uint64_t *full,
@@ -384,18 +431,19 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
 #endif
 
 // paged_tiles.cu: the sequences of minRows query rows per kv head and more, fp16 queries, on tcgen05
-int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st);
+int pagedAttnTiles(const tc_paged_kv *c, const PagedAttnParams &p, cudaStream_t st, uint32_t *blocks);
+// paged_rows.cu: the same for f32 queries over fp16 pages of head_dim 64 and 128
+int pagedAttnRows(const tc_paged_kv *c, const PagedAttnParams &p, cudaStream_t st, uint32_t *blocks);
 constexpr int kPagedSMs = 148;      // blocks that the workspace has room for, per block of an SM
 constexpr uint32_t kPagedTile = 128;  // query rows of a tile of the tiles kernel
 
 // The workspace: two partials per block of the two kernels' widest grids, then what the merge finds per block.
-constexpr size_t kRowsParts = size_t(2) * kPagedSMs * 2 * pagedSlot(64, 128);       // f32
+constexpr size_t kStepsParts = size_t(2) * kPagedSMs * 3 * pagedSlot(16, 128);  // f32
 constexpr size_t kTilesParts = size_t(2) * kPagedSMs * pagedSlot(2 * kPagedTile, 128);
-static_assert(2 * pagedSlot(64, 128) >= pagedSlot(64, 256) && pagedSlot(2 * kPagedTile, 128) >= pagedSlot(kPagedTile, 256), "one block per SM at head_dim 256");
-constexpr size_t kPagedWorkspace = (kRowsParts + kTilesParts) * 4 + size_t(kPagedSMs) * 4 * sizeof(PagedJoin) + 32;
+static_assert(pagedSlot(2 * kPagedTile, 128) >= pagedSlot(kPagedTile, 256), "one query tile at head_dim 256");
+constexpr size_t kPagedWorkspace = (kStepsParts + kTilesParts) * 4 + size_t(kPagedSMs) * 5 * sizeof(PagedJoin) + 32;
 
-// paged_steps.cu: up to pagedStepRows query rows per kv head; *blocks: its grid
-uint32_t pagedStepRows(const tc_paged_kv *c);
+// paged_steps.cu: any sequences, best for few query rows; rows: how many a sequence brings as a rule, for the choice of a form
 int pagedAttnSteps(const tc_paged_kv *c, const PagedAttnParams &p, uint32_t rows, cudaStream_t st, uint32_t *blocks);
 
 int pagedMaps(const tc_paged_kv *c, uint32_t box, CUtensorMap *k, CUtensorMap *v);  // maps of the pools, `box` rows a copy

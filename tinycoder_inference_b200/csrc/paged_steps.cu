@@ -1,6 +1,7 @@
-// paged_steps.cu -- attention of at most 8 or 16 query rows per kv head over a paged cache: decode steps and drafts.
+// paged_steps.cu -- attention of few query rows per kv head over a paged cache: decode steps and drafts, and what f32 queries have of more
+// over int8 pages and at head_dim 256, 16 rows an item.
 //
-// The work, the ring and the partials are paged_attn.cu's; the products have the cache rows on the M side of mma.sync m16n8k16: S^T = K Q^T
+// The work, the ring and the partials are paged_attn.cuh's; the products have the cache rows on the M side of mma.sync m16n8k16: S^T = K Q^T
 // (16 cache rows x 8 query rows) and O^T += V^T P^T (16 dims x 8 query rows), so that 8 query rows fill an instruction and an
 // int8 row is turned into fp16 once for all of a block's query rows.  A warp takes 16 of a tile's 64 rows.  What bounds it is the cache for fp16
 // pages and the conversions of int8 ones (two byte permutes, half an exclusive-or and an fp16 subtraction per two values).
@@ -37,7 +38,7 @@ struct PsL {
     static constexpr int kTotal = kBars + (2 * NST + int(kPaItems)) * 8 + 1024;
     static_assert(NST + 2 <= int(kPaItems), "items");
     static_assert(kBlocks * (kTotal + 1024) <= 228 * 1024, "shared memory of an SM");
-    static_assert(size_t(2) * kPagedSMs * kBlocks * pagedSlot(MR, HD) <= kRowsParts && kBlocks <= 3, "the workspace's room");
+    static_assert(size_t(2) * kPagedSMs * kBlocks * pagedSlot(MR, HD) <= kStepsParts && kBlocks <= 3, "the workspace's room");
 };
 
 template <int HD, bool I8, bool EXACT, int NT>
@@ -89,48 +90,21 @@ pagedStepsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         auto loadQ = [&](uint32_t nt, auto &&put) {
             const uint32_t rr = it.m0 + 8u * nt + n8;
             const bool valid = rr < it.rows;
-            const uint32_t tok = it.token0 + rr / p.group, head = it.kvHead * p.group + rr % p.group;
-            const size_t base = (static_cast<size_t>(tok) * p.nHeads + head) * HD;
             auto dim = [&](int st) { return I8 ? 128 * (st / 8) + 32 * static_cast<int>(c) + 4 * (st % 8) : 64 * (st / 4) + 16 * static_cast<int>(c) + 4 * (st % 4); };
-            float scale = p.scaleLog2;
-            if constexpr (!EXACT) {
+            if constexpr (EXACT) {
+                return p.scaleLog2 * pagedQuery<NS>(p, it, rr, valid, HD, dim, put);
+            } else {
+                const uint32_t tok = it.token0 + rr / p.group, head = it.kvHead * p.group + rr % p.group;
+                const __half *src = static_cast<const __half *>(p.q) + (static_cast<size_t>(tok) * p.nHeads + head) * HD;
 #pragma unroll
                 for (int st = 0; st < NS; ++st) {
                     uint2 x = make_uint2(0u, 0u);
-                    if (valid) x = __ldg(reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + base + dim(st)));
+                    if (valid) x = __ldg(reinterpret_cast<const uint2 *>(src + dim(st)));
                     const uint32_t w[2] = {x.x, x.y};
                     put(st, w);
                 }
-            } else {
-                float4 x[NS];
-                float top = 0.0f;
-#pragma unroll
-                for (int st = 0; st < NS; ++st) {
-                    x[st] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (valid) x[st] = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + base + dim(st)));
-                    top = fmaxf(top, fmaxf(fmaxf(fabsf(x[st].x), fabsf(x[st].y)), fmaxf(fabsf(x[st].z), fabsf(x[st].w))));
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // the row's largest goes to [2^10, 2^11), so that what the upper half leaves is a normal fp16 number
-                float up = 1.0f;
-                if (top > 0.0f && top < INFINITY) {
-                    const int e = min(126, max(-116, static_cast<int>(__float_as_uint(top) >> 23) - 127));
-                    up = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
-                    scale = p.scaleLog2 * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
-                }
-#pragma unroll
-                for (int st = 0; st < NS; ++st) {
-                    float h[4], l[4];
-                    splitHalf(x[st].x * up, h[0], l[0]);
-                    splitHalf(x[st].y * up, h[1], l[1]);
-                    splitHalf(x[st].z * up, h[2], l[2]);
-                    splitHalf(x[st].w * up, h[3], l[3]);
-                    const uint32_t w[4] = {packHalf2(h[0], h[1]), packHalf2(h[2], h[3]), packHalf2(l[0], l[1]), packHalf2(l[2], l[3])};
-                    put(st, w);
-                }
+                return p.scaleLog2;
             }
-            return scale;
         };
         if constexpr (kQRegs) {
             const float s = loadQ(0, [&](int st, const uint32_t(&w)[QW]) {
@@ -429,8 +403,6 @@ static int launchSteps(const CUtensorMap &k, const CUtensorMap &v, const PagedAt
     *blocks = std::min(numSMs(), kPagedSMs) * L::kBlocks;
     return launchDependent(kern, dim3(*blocks), L::kThreads, L::kTotal, st, 1, k, v, p);
 }
-
-uint32_t pagedStepRows(const tc_paged_kv *) { return 16; }
 
 int pagedAttnSteps(const tc_paged_kv *c, const PagedAttnParams &p, uint32_t rows, cudaStream_t st, uint32_t *blocks) {
     CUtensorMap k, v;

@@ -13,6 +13,7 @@
 //   * an int8 store's tiles go through three converter warps (13 - 15) to fp16 integers, exactly; a row's K scale comes to its scores and its V scale to
 //     its probabilities in f32.  The running maximum is then one of score + log2 of the largest V scale of the tile, so what P holds stays below 2^8;
 //   * rows past the sequence may hold anything: scores there are masked by selects, and the warp that issues P V writes zeros over V's.
+#include <algorithm>
 #include <cstring>
 
 #include "paged_attn.cuh"
@@ -701,7 +702,7 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 }
 
 template <int HD, bool I8>
-static int launchTiles(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const PagedAttnParams &p, cudaStream_t st) {
+static int launchTiles(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const PagedAttnParams &p, cudaStream_t st, uint32_t *blocks) {
     using L = PtL<HD, I8>;
     static bool attrDone[64] = {false};
     int dev = 0;
@@ -710,10 +711,11 @@ static int launchTiles(const CUtensorMap &q, const CUtensorMap &k, const CUtenso
         TC_CUDA_OK(cudaFuncSetAttribute((pagedTilesKernel<HD, I8>), cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
         attrDone[dev] = true;
     }
-    return launchDependent(pagedTilesKernel<HD, I8>, dim3(numSMs() < kPagedSMs ? numSMs() : kPagedSMs), L::kThreads, L::kTotal, st, 1, q, k, v, p);
+    *blocks = std::min(numSMs(), kPagedSMs);
+    return launchDependent(pagedTilesKernel<HD, I8>, dim3(*blocks), L::kThreads, L::kTotal, st, 1, q, k, v, p);
 }
 
-int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st) {
+int pagedAttnTiles(const tc_paged_kv *c, const PagedAttnParams &p, cudaStream_t st, uint32_t *blocks) {
     CUtensorMap q, k, v;
     int rc = pagedMaps(c, p.box, &k, &v);
     if (rc != TC_OK) return rc;
@@ -727,9 +729,9 @@ int pagedAttnTiles(const tc_paged_kv *c, PagedAttnParams p, cudaStream_t st) {
     key.rank = 3, key.elemBytes = 2, key.swizzle = 3;
     rc = getTensorMap(key, &q);
     if (rc != TC_OK) return rc;
-    if (c->kvI8) return c->hd == 128 ? launchTiles<128, true>(q, k, v, p, st) : launchTiles<256, true>(q, k, v, p, st);
-    if (c->hd == 64) return launchTiles<64, false>(q, k, v, p, st);
-    return c->hd == 128 ? launchTiles<128, false>(q, k, v, p, st) : launchTiles<256, false>(q, k, v, p, st);
+    if (c->kvI8) return c->hd == 128 ? launchTiles<128, true>(q, k, v, p, st, blocks) : launchTiles<256, true>(q, k, v, p, st, blocks);
+    if (c->hd == 64) return launchTiles<64, false>(q, k, v, p, st, blocks);
+    return c->hd == 128 ? launchTiles<128, false>(q, k, v, p, st, blocks) : launchTiles<256, false>(q, k, v, p, st, blocks);
 }
 
 }  // namespace tc
