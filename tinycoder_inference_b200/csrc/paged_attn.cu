@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(256) pagedMergeKernel(const __grid_constant__ 
     const float *parts = second ? partsB : p.parts;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const size_t slot = pagedSlot(j.mr, HD);
-    auto part = [&](uint32_t c) { return parts + (2u * static_cast<size_t>(from + c) + (c == 0u ? 1u : 0u)) * slot; };
+    auto part = [&](uint32_t c) { return parts + (2u * static_cast<size_t>(from + c * j.groups) + (c == 0u ? 1u : 0u)) * slot; };
     const uint32_t W = j.count <= 8u ? 1u : j.count <= 16u ? 2u : j.count <= 32u ? 4u : 8u, perPass = 8u / W, mine = warp % W;
     const uint32_t rows = min(j.mr, j.rows - j.row0);
     for (uint32_t i0 = blockIdx.y * perPass; i0 < rows; i0 += gridDim.y * perPass) {

@@ -16,10 +16,10 @@ constexpr uint32_t kPaTile = 64;  // cache rows of a unit
 
 // An item that lies in several blocks' runs, as the first of them leaves it for the merge: `count` blocks from this one on; their
 // partials are acc [mr][hd], m [mr], l [mr] (out = sum exp2(m - M) acc / sum exp2(m - M) l), in the first block's second slot -- its
-// run ends with the item -- and the others' first one.  count 0: nothing to join.
+// run ends with the item -- and the others' first one; the k-th of them is block (this one + k groups).  count 0: nothing to join.
 __host__ __device__ constexpr size_t pagedSlot(uint32_t mr, uint32_t hd) { return (static_cast<size_t>(mr) * (hd + 2) + 7) & ~size_t(7); }  // f32
 struct PagedJoin {
-    uint32_t count, row0, rows, token0, kvHead, mr, pad[2];  // rows: of the sequence's kv head; row0: the item's first
+    uint32_t count, row0, rows, token0, kvHead, mr, groups, pad;  // rows: of the sequence's kv head; row0: the item's first
 };
 
 struct PagedAttnParams {
@@ -130,14 +130,18 @@ __device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, const Pag
     return s;
 }
 
-// A walk over a block's run of units, item by item; every warp makes its own, in step.
+// A walk of a producer warp over its block's run of units, item by item.
 struct PagedWalk {
     uint32_t mr, over;        // query rows of an item; units ahead of its tiles that stand for what an item costs beside them
+    // Kv heads whose units lie in a row, and groups of blocks (block b: group b % groups).  Either all heads and one group, or a head
+    // for each of nKV groups: the blocks of a sequence's heads then pass over the same cache rows at the same time, which are
+    // neighbours in memory, and share the scales of an int8 row.
+    uint32_t heads, groups, index;  // index: the block's in its group
     static constexpr uint32_t kHeld = 4;
     PagedRaw raw[kHeld];      // sequences lane, 32 + lane, ..
-    uint64_t total, at, end;  // units of the launch; the block's next and last
-    uint32_t blocks;          // blocks with work
-    uint32_t seq, kvHead, item;
+    uint64_t total, at, end;  // units of the group; the block's next and last
+    uint32_t blocks;          // ... of the group; its blocks with work
+    uint32_t seq, kvHead0, kvHead, item;
     uint64_t item0;           // first unit of the item
     uint32_t tiles;           // its tiles
     PagedSeq s;
@@ -151,7 +155,10 @@ struct PagedWalk {
     // What begin() finds in its first look, before the kernels ahead in the stream are complete: the chain of loads and quotients at a
     // block's start (4 us, most of it instructions that come from far) then passes under them.  As a rule the tables are older than
     // those kernels; start() looks again and begins anew where they were not.
-    __device__ __forceinline__ bool prepare(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
+    __device__ __forceinline__ bool prepare(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead, bool headsApart) {
+        headsApart = headsApart && gridDim.x >= p.c.nKV;
+        heads = headsApart ? 1u : p.c.nKV, groups = headsApart ? p.c.nKV : 1u;
+        index = blockIdx.x / groups, kvHead0 = headsApart ? blockIdx.x - index * groups : 0u;
         look(p, raw);
         return begin(p, itemRows, overhead);
     }
@@ -178,7 +185,7 @@ struct PagedWalk {
     __device__ __forceinline__ bool begin(const PagedAttnParams &p, uint32_t itemRows, uint32_t overhead) {
         mr = itemRows, over = overhead;
         const uint32_t lane = threadIdx.x & 31u;
-        auto unitsOf = [&](uint32_t b, const PagedRaw &r) { return b < p.c.batch ? unitsAll(pagedSeq(p, r), p.group) * p.c.nKV : 0u; };
+        auto unitsOf = [&](uint32_t b, const PagedRaw &r) { return b < p.c.batch ? unitsAll(pagedSeq(p, r), p.group) * heads : 0u; };
         uint64_t held[kHeld], sum = 0;  // units of the first sequences, out of registers; the others are looked up
 #pragma unroll
         for (uint32_t k = 0; k < kHeld; ++k) held[k] = unitsOf(32u * k + lane, raw[k]), sum += held[k];
@@ -187,9 +194,9 @@ struct PagedWalk {
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum;
         if (total == 0u) return false;
-        blocks = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x), total));
-        if (blockIdx.x >= blocks) return false;
-        at = firstOf(blockIdx.x), end = firstOf(blockIdx.x + 1u);
+        blocks = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x / groups), total));
+        if (index >= blocks) return false;
+        at = firstOf(index), end = firstOf(index + 1u);
         // the sequence that holds unit `at`
         uint64_t base = 0;
         bool have = false;
@@ -221,8 +228,8 @@ struct PagedWalk {
         s = pagedSeq(p, found);
         if (s.rows == 0u) return false;  // (only where the tables changed meanwhile)
         uint64_t in = at - base;
-        kvHead = 0;
-        if (p.c.nKV > 1u) {
+        kvHead = kvHead0;
+        if (heads > 1u) {
             const uint64_t per = unitsAll(s, p.group);
             kvHead = static_cast<uint32_t>(divide(in, per));
             in -= kvHead * per;
@@ -252,8 +259,8 @@ struct PagedWalk {
         if (at + over >= end) return false;  // (a run that ends in front of an item's tiles leaves it to the next block)
         if (++item == s.items(mr)) {
             item = 0;
-            if (++kvHead == p.c.nKV) {
-                kvHead = 0;
+            if (++kvHead == kvHead0 + heads) {
+                kvHead = kvHead0;
                 do {
                     if (++seq >= p.c.batch) return false;  // (not reached: the run is not done)
                     s = pagedSeq(p, pagedRaw(p, seq));
@@ -282,7 +289,7 @@ __device__ __forceinline__ uint32_t bytesHi(uint32_t w) { return sub1152(__byte_
 __device__ __forceinline__ void pagedLeaveJoin(const PagedAttnParams &p, const PagedWalk *w, uint32_t count) {
     PagedJoin j;
     j.count = count;
-    if (count != 0u) j.row0 = w->item * w->mr, j.rows = w->s.rows, j.token0 = w->s.token0, j.kvHead = w->kvHead, j.mr = w->mr;
+    if (count != 0u) j.row0 = w->item * w->mr, j.rows = w->s.rows, j.token0 = w->s.token0, j.kvHead = w->kvHead, j.mr = w->mr, j.groups = w->groups;
     p.joins[blockIdx.x] = j;
 }
 // What a block has of an item, as its producer hands it to the consumers: tiles t0 .. t0 + nTiles - 1 of it (nTiles 0: the run is
@@ -346,7 +353,7 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
     PagedWalk w;
     uint32_t handed = 0;  // items
     bool ok = true;
-    const bool some = w.prepare(p, L::MR, 0u);
+    const bool some = w.prepare(p, L::MR, 0u, true);
     gridDepWait();
     gridDepLaunch();
     if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
@@ -360,7 +367,7 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
             it.whole = it.t0 == 0u && t1 == w.tiles, it.part = 0;
             if (!it.whole) {
                 const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
-                it.part = blockIdx.x == c0 ? 1u : 0u;
+                it.part = w.index == c0 ? 1u : 0u;
                 if (it.part) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
             }
             items[handed % kPaItems] = it;
@@ -398,7 +405,7 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
             __syncwarp();
             uint8_t *stage = smem + st * L::kStage;
             if (lane < n) {
-    #pragma unroll
+#pragma unroll
                 for (int h = 0; h < L::kPanels; ++h) {
                     tmaLoad4D(stage + h * L::kPanel + lane * boxBytes, &tmK, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
                     tmaLoad4D(stage + L::kMat + h * L::kPanel + lane * boxBytes, &tmV, &full[st], h * (L::kI8 ? 128 : 64), w.kvHead, in, page);
@@ -406,7 +413,7 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
             }
             if constexpr (L::kI8) {
                 float *sc = reinterpret_cast<float *>(smem + L::kScales) + st * 128u;
-    #pragma unroll
+#pragma unroll
                 for (uint32_t u = 0; u < 2; ++u) {
                     const uint32_t key = lane + 32u * u, from = key / p.box;
                     const uint32_t pg = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, in, from) + key - from * p.box;
