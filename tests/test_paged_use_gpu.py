@@ -169,6 +169,34 @@ def test_pages_far_into_a_pool(ws, io):
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("tokens", [12, 4000])
+def test_tokens_of_no_sequence_are_left(ws, tokens):
+    """`starts` may begin behind the first token and end ahead of the last one."""
+    nKV, hd = 4, 128
+    c = Paged("f16", 8, nKV, hd, [tokens, 40], [tokens - 9, 3], 16, seed=6)
+    c.starts += 4
+    new = tokens - 6
+    q, k = c.normal(tokens, 8, hd), c.normal(tokens, nKV, hd)
+    out, kc = torch.full_like(q, 5.0), c.kc.clone()
+    ops.paged_write(k, k, c.kc, c.vc, c.pages, c.lens, starts=c.starts, q=q, q_out=out)
+    row = torch.cat([c.rows(b, n - m, n) for b, (n, m) in enumerate(zip(c.lens_h, c.new_h))])
+    kc.view(-1, nKV, hd)[row] = k[4:4 + new].half()
+    assert torch.equal(c.kc.view(torch.int16), kc.view(torch.int16))
+    for t, want in ((out, q),):
+        assert torch.equal(t[4:4 + new], want[4:4 + new]) and (t[:4] == 5).all() and (t[4 + new:] == 5).all()
+    ko = torch.full_like(k, 5.0)
+    vo = ko.clone()
+    ops.paged_read(c.kc, c.vc, c.pages, c.lens, ko, vo, starts=c.starts)
+    assert torch.equal(vo[4:4 + new], k[4:4 + new].half().float()) and (vo[:4] == 5).all() and (vo[4 + new:] == 5).all()
+    for io in (torch.float32, torch.float16):
+        out = torch.full((tokens, 8, hd), 5.0, dtype=io, device="cuda")
+        ops.attn_paged(q.to(io), c.kc, c.vc, c.pages, c.lens, out, ws, starts=c.starts)
+        assert (out[:4] == 5).all() and (out[4 + new:] == 5).all()
+        if tokens < 100:
+            c.check(q[4:4 + new].to(io), out[4:4 + new])
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("max_tokens", [0, 1, 7, 1000])
 def test_the_hint_does_not_change_what_is_computed(ws, max_tokens):
     for store, io in (("f16", torch.float16), ("i8", torch.float16), ("f16", torch.float32), ("i8", torch.float32)):

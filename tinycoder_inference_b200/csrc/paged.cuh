@@ -23,7 +23,7 @@ PagedView pagedView(const tc_paged_kv *c, unsigned int *err);
 __device__ __forceinline__ uint32_t seqStart(const PagedView &v, uint32_t b) { return v.starts != nullptr ? __ldg(v.starts + b) : b * v.perSeq; }
 
 // The sequence of token t, found by a group of G lanes that work on the same token (starts ascend: the last b with starts[b] <= t),
-// and the token's position in it.  False: the token lies behind the last sequence.  A position before the first row is negative.
+// and the token's position in it.  False: the token lies behind the last sequence (or ahead of the first).  A position before the first row is negative.
 template <uint32_t G>
 __device__ __forceinline__ bool findToken(const PagedView &v, uint32_t t, uint32_t &seq, int64_t &pos) {
     uint32_t b = 0, end;
@@ -42,7 +42,7 @@ __device__ __forceinline__ bool findToken(const PagedView &v, uint32_t t, uint32
             n = min(step, n - off);
         }
         end = __ldg(v.starts + b + 1u);
-        if (t >= end) return false;
+        if (t >= end || (b == 0u && t < __ldg(v.starts))) return false;
     }
     seq = b;
     pos = static_cast<int64_t>(__ldg(v.lens + b)) - static_cast<int64_t>(end - t);

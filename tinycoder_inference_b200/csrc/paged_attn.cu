@@ -172,7 +172,7 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
     unsigned int *err = devErrorWord();
     TC_REQUIRE(err != nullptr, TC_ECUDA, "no CUDA device");
     const uint32_t most = c->starts != nullptr ? c->tokens : c->tokens / c->batch;
-    if (maxTokens == 0 || maxTokens > most) maxTokens = most;
+    if (maxTokens == 0 || maxTokens > most || c->starts == nullptr) maxTokens = most;
     const uintptr_t base = (reinterpret_cast<uintptr_t>(workspace) + 31) & ~uintptr_t(31);
     PagedAttnParams p;
     p.c = pagedView(c, err);

@@ -162,8 +162,8 @@ struct PagedWalk {
         look(p, raw);
         return begin(p, itemRows, overhead);
     }
-    // Behind the wait for those kernels.  some: what prepare() said.
-    __device__ __forceinline__ bool start(const PagedAttnParams &p, bool some) {
+    // Behind the wait for those kernels.  some: what prepare() said; kept: it stands.
+    __device__ __forceinline__ bool start(const PagedAttnParams &p, bool some, bool &kept) {
         PagedRaw now[kHeld];
         look(p, now);
         const uint32_t lane = threadIdx.x & 31u;
@@ -173,7 +173,8 @@ struct PagedWalk {
         bool same = p.c.batch <= 32u * kHeld;
 #pragma unroll
         for (uint32_t k = 0; k < kHeld; ++k) same = same && now[k] == raw[k], raw[k] = now[k];
-        return __all_sync(0xffffffffu, same) ? some : begin(p, mr, over);
+        kept = __all_sync(0xffffffffu, same);
+        return kept ? some : begin(p, mr, over);
     }
     __device__ __forceinline__ void look(const PagedAttnParams &p, PagedRaw (&r)[kHeld]) const {
         const uint32_t lane = threadIdx.x & 31u;
@@ -357,8 +358,28 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
     gridDepWait();
     gridDepLaunch();
     if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
-    if (w.start(p, some)) do {
-        const int32_t *table = p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq;
+    // Where this lane's box of a tile lies: looked up a tile ahead, and the first one's entry on its way beside the second look at the
+    // tables.
+    struct At {
+        uint32_t have, in;
+        int32_t page;
+    };
+    auto look = [&](uint32_t t) {
+        const uint32_t row0 = t * kPaTile;
+        At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
+        if (lane < at.have) {
+            const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
+            at.in = row - slot * p.c.pageRows;
+            at.page = __ldg(p.c.pages + static_cast<size_t>(w.seq) * p.c.pagesPerSeq + slot);
+        }
+        return at;
+    };
+    At next{0u, 0u, 0};
+    if (some) next = look(w.first());
+    bool kept;
+    const bool work = w.start(p, some, kept);
+    if (work && !kept) next = look(w.first());
+    if (work) do {
         const uint32_t t1 = w.last();
         if (lane == 0) {
             PaItem it;
@@ -374,22 +395,7 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
             mbarArrive(&itemFull[handed % kPaItems]);
         }
         ++handed;
-        // where this lane's box of a tile lies: looked up a tile ahead
-        struct At {
-            uint32_t have, in;
-            int32_t page;
-        };
-        auto look = [&](uint32_t t) {
-            const uint32_t row0 = t * kPaTile;
-            At at{w.s.len > row0 ? min(boxes, (w.s.len - row0 + p.box - 1u) / p.box) : 0u, 0u, 0};
-            if (lane < at.have) {
-                const uint32_t row = row0 + lane * p.box, slot = row / p.c.pageRows;
-                at.in = row - slot * p.c.pageRows;
-                at.page = __ldg(table + slot);
-            }
-            return at;
-        };
-        At next = look(w.first());
+        if (handed > 1u) next = look(w.first());
         for (uint32_t t = w.first(); t < t1; ++t, ++g) {
             const uint32_t n = next.have, in = next.in;
             uint32_t page = static_cast<uint32_t>(next.page);

@@ -237,7 +237,7 @@ constexpr uint32_t kReadTokens = 32;
 template <int HD, bool I8, bool HALF>
 __global__ void __launch_bounds__(256) pagedReadManyKernel(const __grid_constant__ PagedReadParams p) {
     constexpr uint32_t E = I8 ? 16 : 8, G = HD / E, U = 4;
-    __shared__ int64_t rowS[kReadTokens];  // -1: no page; -2: behind the last sequence
+    __shared__ int64_t rowS[kReadTokens];  // -1: no page; -2: of no sequence
     gridDepWait();
     gridDepLaunch();
     const uint32_t t0 = blockIdx.x * kReadTokens;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(256) pagedReadManyKernel(const __grid_constant
         const uint32_t t = t0 + threadIdx.x;
         int64_t at = -2;
         if (t < p.c.tokens) {
-            uint32_t b = 0, n = p.c.batch, end;
+            uint32_t b = 0, n = p.c.batch, end, first = 0;
             if (p.c.starts == nullptr) {
                 b = t / p.c.perSeq, end = (b + 1u) * p.c.perSeq;
             } else {
@@ -255,8 +255,9 @@ __global__ void __launch_bounds__(256) pagedReadManyKernel(const __grid_constant
                     b += right ? half : 0u, n = right ? n - half : half;
                 }
                 end = __ldg(p.c.starts + b + 1u);
+                if (b == 0u) first = __ldg(p.c.starts);
             }
-            if (t < end) {
+            if (t >= first && t < end) {
                 size_t row;
                 at = pagedRow(p.c, b, static_cast<int64_t>(__ldg(p.c.lens + b)) - static_cast<int64_t>(end - t), row) ? static_cast<int64_t>(row) : -1;
                 if (at < 0) atomicOr(p.c.err, kDevErrRowBound);

@@ -26,12 +26,13 @@ struct PsL {
     static constexpr int kMat = kPanels * kPanel;
     static constexpr int kStage = 2 * kMat;
     static constexpr int kBlocks = HD == 256 ? (I8 && NT == 1 ? 2 : 1) : kStage == 16384 && NT == 1 ? 3 : 2;
-    static constexpr int NST = kStage == 65536 ? (NT > 1 ? 2 : 3) : kStage == 32768 ? (kBlocks == 1 ? 5 : NT > 1 ? 2 : 3) : kBlocks == 3 ? 4 : 5;
+    static constexpr int NST = kStage == 65536 ? (NT > 1 ? 2 : 3) : kStage == 32768 ? (kBlocks == 1 ? 5 : NT > 1 ? 2 : 3) : kBlocks == 3 ? (HD == 64 ? 4 : 3) : 5;
     static constexpr int NS = HD / 16;
     static constexpr int kScales = NST * kStage;                              // [stage][K, V][64]
     static constexpr int kQ = kScales + (I8 ? NST * 512 : 0);                 // NT > 1: [n tile][step][lane] hi (lo) pairs
     static constexpr int kBuf = kQ + (NT > 1 ? NT * NS * 32 * (EXACT ? 16 : 8) : 0);
-    static constexpr int kMl = kBuf + NW * MR * 36 * 4;                       // [warp][row] (m, l)
+    static constexpr int kPass = NT == 1 && I8 && HD == 128 ? 128 : 32;      // dims that the warps put together at a time
+    static constexpr int kMl = kBuf + NW * MR * (kPass + 4) * 4;              // [warp][row] (m, l)
     static constexpr int kRowScale = kMl + NW * MR * 8;
     static constexpr int kItems = kRowScale + MR * 4;
     static constexpr int kBars = (kItems + int(kPaItems * sizeof(PaItem)) + 7) / 8 * 8;
@@ -358,28 +359,35 @@ pagedStepsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             if (I8) f[r] *= __uint_as_float(static_cast<uint32_t>(127 + vexp) << 23);
             if (!whole && warp == 0 && n8 == 0) part[MR * HD + row] = M, part[MR * HD + MR + row] = sum;
         }
-        // 32 dims at a time through shared memory
+        // kPass dims at a time through shared memory
+        constexpr int PW = L::kPass, PT = PW / 16;  // 16-dim tiles of a pass
+        constexpr uint32_t kRow = PW + 4;
 #pragma unroll
-        for (int pass = 0; pass < NM / 2; ++pass) {
+        for (int pass = 0; pass < NM / PT; ++pass) {
             if (pass > 0) namedBarSync(1, 128);
-            float *b = buf + warp * (MR * 36u);
+            float *b = buf + warp * (MR * kRow);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj)
+                for (int jj = 0; jj < PT; ++jj)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        b[(8u * nt + 2u * c + (e & 1)) * 36u + (I8 ? n8 * 4u + 2u * jj + (e >> 1) : 16u * jj + 8u * (e >> 1) + n8)] = o[nt][2 * pass + jj][e] * f[2 * nt + (e & 1)];
+                    for (int e = 0; e < 4; ++e) {
+                        // int8: a pass of 32 dims has four of each 16 (a thread's quads), one of 128 has all of a panel
+                        const uint32_t col = !I8       ? 16u * jj + 8u * (e >> 1) + n8
+                                             : PW == 32 ? n8 * 4u + 2u * jj + (e >> 1)
+                                                        : n8 * 16u + 2u * jj + (e >> 1);
+                        b[(8u * nt + 2u * c + (e & 1)) * kRow + col] = o[nt][PT * pass + jj][e] * f[2 * nt + (e & 1)];
+                    }
             namedBarSync(1, 128);
-            for (uint32_t i = threadIdx.x; i < MR * 8u; i += 128u) {
-                const uint32_t row = i >> 3, q4 = i & 7u, r = it.m0 + row;
+            for (uint32_t i = threadIdx.x; i < MR * (PW / 4); i += 128u) {
+                const uint32_t row = i / (PW / 4), q4 = i % (PW / 4), r = it.m0 + row;
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (uint32_t k = 0; k < 4u; ++k) {
-                    const float4 y = *reinterpret_cast<const float4 *>(buf + k * (MR * 36u) + row * 36u + q4 * 4u);
+                    const float4 y = *reinterpret_cast<const float4 *>(buf + k * (MR * kRow) + row * kRow + q4 * 4u);
                     x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
                 }
-                const uint32_t dim = I8 ? 128u * (pass / 4) + 16u * q4 + 4u * (pass % 4) : 32u * pass + 4u * q4;
+                const uint32_t dim = I8 && PW == 32 ? 128u * (pass / 4) + 16u * q4 + 4u * (pass % 4) : PW * pass + 4u * q4;
                 if (r >= it.rows) continue;
                 if (whole) pagedStore(p, HD, it.token0, it.kvHead, r, dim, x);
                 else __stcg(reinterpret_cast<float4 *>(part + row * HD + dim), x);

@@ -247,8 +247,8 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         gridDepWait();
         gridDepLaunch();
         if (lane == 0) pagedLeaveJoin(p, nullptr, 0u);
-        bool ok = true;
-        if (w.start(p, some)) do {
+        bool ok = true, kept;
+        if (w.start(p, some, kept)) do {
             uint32_t joins;
             const PtItem it = ptItem<kOne>(p, w, joins);
             if (lane == 0) {
