@@ -248,10 +248,9 @@ struct PagedWalk {
         tiles = s.tiles(mr, item, p.group);
         return end - item0 > over;
     }
-    // Tiles [first, last) of the item are the block's; tiles of the item's first and last block.
+    // Tiles [first, last) of the item are the block's; the group's block that has its last one.
     __device__ __forceinline__ uint32_t first() const { return at - item0 > over ? static_cast<uint32_t>(at - item0 - over) : 0u; }
     __device__ __forceinline__ uint32_t last() const { return static_cast<uint32_t>(min(end - item0, static_cast<uint64_t>(tiles) + over)) - over; }
-    __device__ __forceinline__ uint32_t firstBlock() const { return blockOf(item0 + over); }
     __device__ __forceinline__ uint32_t lastBlock() const { return blockOf(item0 + over + tiles - 1u); }
     // On to the next item; false: the run is done.
     __device__ __forceinline__ bool next(const PagedAttnParams &p) {
@@ -385,12 +384,7 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
             PaItem it;
             it.t0 = w.first(), it.nTiles = t1 - it.t0, it.m0 = w.item * L::MR, it.rows = w.s.rows, it.token0 = w.s.token0;
             it.kvHead = w.kvHead, it.len = w.s.len, it.before = w.s.before;
-            it.whole = it.t0 == 0u && t1 == w.tiles, it.part = 0;
-            if (!it.whole) {
-                const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
-                it.part = w.index == c0 ? 1u : 0u;
-                if (it.part) pagedLeaveJoin(p, &w, c1 - c0 + 1u);
-            }
+            it.whole = it.t0 == 0u && t1 == w.tiles, it.part = it.t0 == 0u ? 1u : 0u;  // (the item's first block uses its second slot)
             items[handed % kPaItems] = it;
             mbarArrive(&itemFull[handed % kPaItems]);
         }
@@ -432,6 +426,8 @@ __device__ __forceinline__ void pagedProduce(const PagedAttnParams &p, const CUt
                 cpAsyncMbarArriveNoinc(&full[st]);
             }
         }
+        // (the quotient waits until the tiles are on their way)
+        if (lane == 0 && w.first() == 0u && t1 != w.tiles) pagedLeaveJoin(p, &w, w.lastBlock() - w.index + 1u);
     } while (ok && w.next(p));
     if (lane == 0) {
         items[handed % kPaItems].nTiles = 0u;

@@ -63,12 +63,8 @@ __device__ __forceinline__ PtItem ptItem(const PagedAttnParams &p, const PagedWa
         it.nB = it.rowsB != 0u ? it.nTiles : 0u;
     }
     it.seq = w.seq, it.kvHead = w.kvHead, it.token0 = w.s.token0, it.len = w.s.len, it.before = w.s.before;
-    it.part = 0, joins = 0, it.pad = 0;
-    if (!it.whole) {
-        const uint32_t c0 = w.firstBlock(), c1 = w.lastBlock();
-        it.part = w.index == c0 ? 1u : 0u;
-        if (w.index == c0) joins = c1 - c0 + 1u;
-    }
+    it.part = it.t0 == 0u ? 1u : 0u, it.pad = 0;  // (the item's first block uses its second slot)
+    joins = it.part && !it.whole ? w.lastBlock() - w.index + 1u : 0u;
     return it;
 }
 
