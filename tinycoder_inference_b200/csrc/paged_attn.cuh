@@ -1,10 +1,11 @@
 // paged_attn.cuh -- attention over a paged cache: the call as its kernels see it and how it is cut into work.
 //
 // An item is up to MR consecutive query rows of one kv head of one sequence; query row r of a sequence's kv head is q head
-// r % group of its token r / group, so the heads that share K and V sit side by side and one pass over the rows serves them.  A
-// unit is one tile of kPaTile cache rows of an item.  The units of all items in a row -- sequence, kv head, rows -- are cut into
-// equal runs, one per block (an item counts some units more than its tiles, for what it costs beside them): ragged lengths, single tokens and prompts fill the SMs alike.  An item that lies in several runs
-// is put together by a second launch from partials in the workspace.
+// r % group of its token r / group, so the heads that share K and V sit side by side and one pass over the rows serves them.
+// A unit is one tile of kPaTile cache rows of an item.  The units of all items in a row -- sequence after sequence -- are cut
+// into equal runs, one per block: ragged lengths, single tokens and prompts fill the SMs alike.  An item that lies in several
+// runs is put together by a second launch from partials in the workspace.  Everything is found on the device, from the tables,
+// so a captured call follows them.
 #pragma once
 
 #include "paged.cuh"
@@ -14,10 +15,11 @@ namespace tc {
 
 constexpr uint32_t kPaTile = 64;  // cache rows of a unit
 
-// An item that lies in several blocks' runs, as the first of them leaves it for the merge: `count` blocks from this one on; their
-// partials are acc [mr][hd], m [mr], l [mr] (out = sum exp2(m - M) acc / sum exp2(m - M) l), in the first block's second slot -- its
-// run ends with the item -- and the others' first one; the k-th of them is block (this one + k groups).  count 0: nothing to join.
-__host__ __device__ constexpr size_t pagedSlot(uint32_t mr, uint32_t hd) { return (static_cast<size_t>(mr) * (hd + 2) + 7) & ~size_t(7); }  // f32
+// A partial: acc [mr][hd], m [mr], l [mr]; out = sum exp2(m - M) acc / sum exp2(m - M) l.  In f32 numbers.
+__host__ __device__ constexpr size_t pagedSlot(uint32_t mr, uint32_t hd) { return (static_cast<size_t>(mr) * (hd + 2) + 7) & ~size_t(7); }
+// An item that lies in several blocks' runs, as the first of them leaves it for the merge: `count` blocks, the k-th of them block
+// (this one + k groups).  The first block's partial is in its second slot -- its run ends with the item -- and the others' in
+// their first one.  count 0: nothing to join.
 struct PagedJoin {
     uint32_t count, row0, rows, token0, kvHead, mr, groups, pad;  // rows: of the sequence's kv head; row0: the item's first
 };
@@ -118,7 +120,8 @@ __device__ __forceinline__ PagedRaw pagedRaw(const PagedAttnParams &p, uint32_t 
     r.len = __ldcg(p.c.lens + b);
     return r;
 }
-__device__ __forceinline__ uint32_t pagedMost(const PagedAttnParams &p) { return p.c.pagesPerSeq * p.c.pageRows; }  // rows that a sequence has pages for
+// rows that a sequence has pages for
+__device__ __forceinline__ uint32_t pagedMost(const PagedAttnParams &p) { return p.c.pagesPerSeq * p.c.pageRows; }
 __device__ __forceinline__ PagedSeq pagedSeq(const PagedAttnParams &p, const PagedRaw &r) {
     const uint32_t stop = min(r.stop, p.c.tokens), n = stop > r.start ? stop - r.start : 0u;
     PagedSeq s;
