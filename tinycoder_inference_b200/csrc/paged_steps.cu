@@ -28,13 +28,15 @@ struct PsL {
     static constexpr int kPanel = int(kPaTile) * 128;
     static constexpr int kMat = kPanels * kPanel;
     static constexpr int kStage = 2 * kMat;
-    // (head_dim 256 with f32 results spills at two blocks: 64 sessions of 16 / 2 / 256 over int8 pages 79 us, with one 72)
-    static constexpr int kBlocks = HD == 256 ? (I8 && NT == 1 && !EXACT ? 2 : 1) : kStage == 16384 && NT == 1 ? 3 : 2;
+    static constexpr bool kQRegs = NT == 1 && !(HD == 256 && EXACT);           // q in registers, else in shared memory
+    // (in registers head_dim 256 with f32 results spills at two blocks per SM: 64 sessions of 16 / 2 / 256 over int8 pages 79 us, one block
+    // 72, two with q in shared memory 64)
+    static constexpr int kBlocks = HD == 256 ? (I8 && NT == 1 ? 2 : 1) : kStage == 16384 && NT == 1 ? 3 : 2;
     static constexpr int NST = kStage == 65536 ? (NT > 1 ? 2 : 3) : kStage == 32768 ? (kBlocks == 1 ? 5 : NT > 1 ? 2 : 3) : kBlocks == 3 ? (HD == 64 ? 4 : 3) : 5;
     static constexpr int NS = HD / 16;
     static constexpr int kScales = NST * kStage;                              // [stage][K, V][64]
     static constexpr int kQ = kScales + (I8 ? NST * 512 : 0);                 // NT > 1: [n tile][step][lane] hi (lo) pairs
-    static constexpr int kBuf = kQ + (NT > 1 ? NT * NS * 32 * (EXACT ? 16 : 8) : 0);
+    static constexpr int kBuf = kQ + (kQRegs ? 0 : NT * NS * 32 * (EXACT ? 16 : 8));
     static constexpr int kPass = NT == 1 && I8 && HD == 128 ? 128 : 32;      // dims that the warps put together at a time
     static constexpr int kMl = kBuf + NW * MR * (kPass + 4) * 4;              // [warp][row] (m, l)
     static constexpr int kRowScale = kMl + NW * MR * 8;
@@ -77,7 +79,7 @@ pagedStepsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 
     const uint32_t c = lane & 3u, n8 = lane >> 2, key0 = warp * 16u;
     constexpr int NS = L::NS, NM = HD / 16, QW = EXACT ? 4 : 2;  // steps of q . K; 16-dim output tiles; registers of a step's q
-    constexpr bool kQRegs = NT == 1;
+    constexpr bool kQRegs = L::kQRegs;
     float *buf = reinterpret_cast<float *>(smem + L::kBuf), *rowScaleS = reinterpret_cast<float *>(smem + L::kRowScale);
     float2 *ml = reinterpret_cast<float2 *>(smem + L::kMl);
     uint32_t *qS = reinterpret_cast<uint32_t *>(smem + L::kQ);
@@ -420,7 +422,10 @@ int pagedAttnSteps(const tc_paged_kv *c, const PagedAttnParams &p, uint32_t rows
     CUtensorMap k, v;
     const int rc = pagedMaps(c, p.box, &k, &v);
     if (rc != TC_OK) return rc;
-#define TC_PAGED_NT(HD, I8, EXACT) (rows <= 8 ? launchSteps<HD, I8, EXACT, 1>(k, v, p, st, blocks) : launchSteps<HD, I8, EXACT, 2>(k, v, p, st, blocks))
+    // One group of 8 query rows an item or two: two share a converted tile, one leaves room for twice the warps.  Drafts of 16 - 48
+    // rows of 16 / 2 / 256 with f32 results: int8 pages 63 us with two, 58 with one; fp16 pages 77 and 79.
+    const bool one = rows <= 8 || (rows <= 64 && c->kvI8 && c->hd == 256 && !p.half);
+#define TC_PAGED_NT(HD, I8, EXACT) (one ? launchSteps<HD, I8, EXACT, 1>(k, v, p, st, blocks) : launchSteps<HD, I8, EXACT, 2>(k, v, p, st, blocks))
 #define TC_PAGED_STEPS(HD, I8) (p.half ? TC_PAGED_NT(HD, I8, false) : TC_PAGED_NT(HD, I8, true))
     if (c->kvI8) return c->hd == 128 ? TC_PAGED_STEPS(128, true) : TC_PAGED_STEPS(256, true);
     if (c->hd == 64) return TC_PAGED_STEPS(64, false);
