@@ -188,6 +188,7 @@ int tc_attn_paged(const tc_paged_kv *c, const void *q, void *out, int half, uint
     p.out32 = (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
     p.scaleLog2 = invSqrt * kLog2e;
     p.half = half != 0;
+    p.zero = 0;
     const uint32_t rows = maxTokens * p.group;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint32_t few = fewRows(c, half != 0);

@@ -37,6 +37,7 @@ struct PagedAttnParams {
     uint32_t minRows, maxRows;    // the kernel takes the sequences with so many query rows per kv head (minRows .. maxRows)
     float scaleLog2;
     int half;                // q and out are fp16
+    uint32_t zero;           // 0 (releaseStage)
 };
 
 #ifdef __CUDACC__
@@ -343,6 +344,15 @@ __device__ __forceinline__ float pagedQuery(const PagedAttnParams &p, const PaIt
         put(st, w);
     }
     return back;
+}
+
+// Hands a stage back once the warp's loads from it have returned.  The arrival alone does not wait for them: with loads still under way it
+// overtook them, and TMA wrote the next tile under the last ldmatrix of the slowest warp (seen as results that differ in a few
+// weights from run to run).  `used` is made of every product that took data of the stage, so that the arrival's address waits for it; zero is
+// a 0 that the compiler does not know.
+__device__ __forceinline__ void releaseStage(uint64_t *bar, uint32_t used, uint32_t zero) {
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0u) mbarArrive(bar + (used & zero));
 }
 
 // The producer warp of the kernels whose consumers share a tile's rows (paged_rows.cu, paged_steps.cu): hands on the items of the block's run

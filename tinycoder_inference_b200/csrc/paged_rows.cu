@@ -167,8 +167,10 @@ pagedRowsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     product(j + 1, r2, r3);
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbarArrive(&empty[st]);
+            uint32_t used = 0u;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) used ^= __float_as_uint(o[j][0]);
+            releaseStage(&empty[st], used, p.zero);
         }
         // ---- the rows out, or into the item's partial ----
         l += __shfl_xor_sync(0xffffffffu, l, 1);

@@ -335,8 +335,12 @@ pagedStepsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                     product(j, r0, r2, r1, r3);
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbarArrive(&empty[st]);
+            uint32_t used = 0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < NM; ++j) used ^= __float_as_uint(o[nt][j][0]);
+            releaseStage(&empty[st], used, p.zero);
         }
 
         // ---- the four warps' shares ----
