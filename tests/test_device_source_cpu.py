@@ -40,3 +40,24 @@ def test_tensor_memory_is_given_back_behind_the_warps_that_issue():
             if barrier.group(1):
                 assert "namedBarArrive(kIssuedBar, " in "\n".join(lines[:i]), (name, i + 1)
     assert found >= 2
+
+
+def _roles(name, *marks):
+    """The code of a kernel's roles: what stands between one mark and the next."""
+    code = _code(name)
+    at = [code.index(m) for m in marks]
+    assert at == sorted(at), name
+    return [code[a:b] for a, b in zip(at, at[1:] + [len(code)])]
+
+
+def test_paged_tiles_wait_for_the_last_release_of_every_slot():
+    """A release of a K or V slot arrives when the products behind it are complete, at a barrier in the block's own memory: somebody
+    has to wait for the last ones before the block leaves, over either kind of pages.  The waiting warp has to have seen the
+    slot's last tile come in, or a parity wait may take an older phase for the last one: over fp16 pages the producers, which
+    wait for every release themselves, over int8 ones the issuing warps, which wait for every tile."""
+    producer, values, converters, issuers, softmax = _roles(
+        "paged_tiles.cu", "if (warp == 8) {", "else if (!I8 && warp == 13)", "else if (I8 && warp >= 13)", "else if (warp >= 9 && warp < 13)", "else if (!(kOne && warp >= 4))")
+    assert "drain(kEmpty, gk, NK" in producer and "drain(vEmpty, gv, NV" in values
+    behind = issuers[issuers.index("g += it.nTiles;"):]
+    assert re.search(r"if \(I8 && ok && x == 0u\)", behind)
+    assert "drain(kEmpty, g, NK" in behind and "drain(vEmpty, g, NV" in behind

@@ -475,6 +475,12 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             for (uint32_t tt = t >= 2u ? t - 2u : 0u; tt < t; ++tt)
                 if (!pfWait<kCall>(&pvBuf[2u * x + (tt & 1u)], (tt >> 1) & 1u, err, kDevErrMmaWait)) break;
         }
+        // ... and the last releases of the slots.  Over int8 pages these warps wait for them: a converter knows of its own panels only, and a
+        // parity wait on a slot whose last tile is not in yet would find an older phase.  (These have waited for every tile.)
+        if (I8 && ok && x == 0u) {
+            if (pvRole) drain(vEmpty, g, NV, kDevErrEmptyWait);
+            else drain(kEmpty, g, NK, kDevErrEmptyWait);
+        }
     } else if (!(kOne && warp >= 4)) {
         // --------------------------------- softmax ---------------------------------
         const uint32_t x = warp >> 2;                         // which query tile this warpgroup owns
