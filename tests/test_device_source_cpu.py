@@ -61,3 +61,12 @@ def test_paged_tiles_wait_for_the_last_release_of_every_slot():
     behind = issuers[issuers.index("g += it.nTiles;"):]
     assert re.search(r"if \(I8 && ok && x == 0u\)", behind)
     assert "drain(kEmpty, g, NK" in behind and "drain(vEmpty, g, NV" in behind
+
+
+def test_prefill_commits_to_no_barrier_that_nobody_waits_for():
+    """At head_dim 256 (kAhead) the softmax threads go by pvBuf: a commit to pvDone would be an arrival that no wait sees before the
+    block leaves."""
+    code = _code("prefill_f16.cu")
+    assert re.search(r"kAhead\s*\?\s*pfWait<kCall>\(&pvBuf", code)
+    commits = re.findall(r"[^\n]*umaCommit\(&pvDone\[x\]\)[^\n]*", code)
+    assert len(commits) == 1 and "if (!kAhead)" in commits[0]

@@ -618,7 +618,7 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             for (uint32_t ks = 0; ks < BN / 16; ++ks)  // 16 tokens per step: 8 columns of fp16 P, 2 KB of V
                                 umaMmaTS(tO, tP + ks * 8u, descAdvance(dV, ks * 2048u), idPV, (tt > t || ks > 0) ? 1u : 0u);
                             umaCommit(&pvBuf[2u * x + (tt & 1u)]);
-                            umaCommit(&pvDone[x]);
+                            if (!kAhead) umaCommit(&pvDone[x]);  // (with it the softmax goes by pvBuf)
                             umaCommit(&vEmpty[s]);
                             PF_STAMP(4u + x, j, 2);
                         }
@@ -729,7 +729,8 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 // complete (the next one cannot start before this thread publishes P).  The last
                 // step takes the wait in any case: a parity wait can only tell the current phase from
                 // the one before it, and the final wait below must not find the barrier two behind.
-                // (pvDone completes one phase per tile, so its parity follows the running count.)
+                // (pvDone completes one phase per tile, so its parity follows the running count; with kAhead a buffer's barrier
+                // completes one per two tiles, and the wait above has seen the phase before.)
                 if (j > 0 && (rescale || j + 1u == myTiles)) {
                     if (!pvWait(tt - 1u)) {
                         ok = false;
