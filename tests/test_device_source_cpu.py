@@ -70,3 +70,15 @@ def test_prefill_commits_to_no_barrier_that_nobody_waits_for():
     assert re.search(r"kAhead\s*\?\s*pfWait<kCall>\(&pvBuf", code)
     commits = re.findall(r"[^\n]*umaCommit\(&pvDone\[x\]\)[^\n]*", code)
     assert len(commits) == 1 and "if (!kAhead)" in commits[0]
+
+
+def test_the_query_tiles_last_release_is_waited_for():
+    """The score warps commit to qFree with an item's last product; the producer waits for it ahead of the next item, so the last
+    item's needs a wait of its own, in the producer, behind its loop over the items."""
+    for name, loop in (("prefill_f16.cu", "item = next;"), ("paged_tiles.cu", "while (ok && w.next(p));")):
+        code = _code(name)
+        producer = code[code.index("if (warp == 8) {"):]
+        behind = producer[producer.index(loop):]
+        behind = behind[:re.search(r"else if \((!I8 && warp == 13|warp >= 9)\)", behind).start()]
+        for x in "01":
+            assert re.search(r"pfWait<kCall>\(&qFree\[%s\], \(n - 1u\) & 1u" % x, behind), (name, x)

@@ -290,6 +290,8 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             items[n % kPtItems].nTiles = 0u;
             mbarArrive(&itemFull[n % kPtItems]);
         }
+        if (ok && n != 0u)  // the query tiles' last release, like those of the slots
+            ok = pfWait<kCall>(&qFree[0], (n - 1u) & 1u, err, kDevErrEmptyWait) && (kOne || pfWait<kCall>(&qFree[1], (n - 1u) & 1u, err, kDevErrEmptyWait));
         if (!ok && n != 0u) pfWait<kCall>(qFull, (n - 1u) & 1u, err, kDevErrFullWait);
         if constexpr (I8) {
             if (!ok || !drain(stEmpty, gs, NS ? NS : 1u, kDevErrEmptyWait)) drain(stFull, gs, NS ? NS : 1u, kDevErrFullWait);

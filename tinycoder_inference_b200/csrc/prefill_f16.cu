@@ -462,7 +462,7 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (warp == 8) {
         // ------------------------ TMA producer and scheduler ------------------------
         if (lane == 0) {
-            uint32_t item = SHARED ? blockIdx.x / share : blockIdx.x, gk = 0, gv = 0;  // gk / gv: K / V tiles requested so far, over all items
+            uint32_t item = SHARED ? blockIdx.x / share : blockIdx.x, n = 0, gk = 0, gv = 0;  // items done; gk / gv: K / V tiles requested so far, over all items
             gridDepWait();  // the twins and the work counter come from the launch in front
             gridDepLaunch();
             itemSlots[0] = item;
@@ -488,7 +488,7 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 ++gv;
                 return true;
             };
-            for (uint32_t n = 0; ok && item < p.totalItems; ++n) {
+            for (; ok && item < p.totalItems; ++n) {
                 const PfItem it = pfItem<SHARED>(p, item);
                 if (SHARED && it.nTiles == 0u) break;  // (nothing is loaded: the block's part of the cluster's end is all there is)
                 PF_BLK(0);
@@ -529,7 +529,10 @@ prefillF16Kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 mbarArrive(&itemFull[(n + 1u) & 3u]);
                 item = next;
             }
-            // the last release of every slot has to have arrived before the block leaves
+            // the last release of every slot, and of the query tiles, has to have arrived before the block leaves
+            if (ok && n != 0u)
+                ok = pfWait<kCall>(&qFree[0], (n - 1u) & 1u, p.err, kDevErrEmptyWait) &&
+                     (kOne || pfWait<kCall>(&qFree[1], (n - 1u) & 1u, p.err, kDevErrEmptyWait));
             for (uint32_t back = 0; ok && back < NK && back < gk; ++back) {
                 const uint32_t g = gk - 1u - back;
                 ok = pfWait<kCall>(&kEmpty[g % NK], (g / NK) & 1u, p.err, kDevErrEmptyWait);
