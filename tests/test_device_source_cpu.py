@@ -82,3 +82,12 @@ def test_the_query_tiles_last_release_is_waited_for():
         behind = behind[:re.search(r"else if \((!I8 && warp == 13|warp >= 9)\)", behind).start()]
         for x in "01":
             assert re.search(r"pfWait<kCall>\(&qFree\[%s\], \(n - 1u\) & 1u" % x, behind), (name, x)
+
+
+def test_int8_decode_releases_only_stages_that_are_filled_again():
+    """A stage's release is waited for by the request of the tile that takes it next.  Where there is none, nobody waits, and the
+    arrival may come after the block has left: there is no commit then."""
+    code = _code("decode_i8_tc.cu")
+    assert len(re.findall(r"mbarWait<true>\(&emptyBar\[", code)) == 1 and "if (it >= NS && !mbarWait<true>(&emptyBar[s]" in code
+    commits = re.findall(r"[^\n]*umaCommit\(&emptyBar\[s\]\)[^\n]*", code)
+    assert len(commits) == 1 and "if (j + NS < nTiles)" in commits[0]

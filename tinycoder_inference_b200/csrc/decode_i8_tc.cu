@@ -473,8 +473,9 @@ decodeI8TcKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                         tcMmaI8(tO, dV + ((k * 4096u) >> 4), dP + ((k * 1024u) >> 4), idPV, k > 0 ? 1u : 0u);
                     umaCommit(&oFull[2u * w + bb]);
                     // K and V of the stage are consumed once these products are done (the score product
-                    // of the tile completed before its P could be written)
-                    umaCommit(&emptyBar[s]);
+                    // of the tile completed before its P could be written).  A release that no later tile waits for is not
+                    // committed: it could arrive behind the block's end.
+                    if (j + NS < nTiles) umaCommit(&emptyBar[s]);
                 }
                 __syncwarp();
                 if (lane == 0) TC_STAMP(16);
