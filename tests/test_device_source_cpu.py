@@ -91,3 +91,17 @@ def test_int8_decode_releases_only_stages_that_are_filled_again():
     assert len(re.findall(r"mbarWait<true>\(&emptyBar\[", code)) == 1 and "if (it >= NS && !mbarWait<true>(&emptyBar[s]" in code
     commits = re.findall(r"[^\n]*umaCommit\(&emptyBar\[s\]\)[^\n]*", code)
     assert len(commits) == 1 and "if (j + NS < nTiles)" in commits[0]
+
+
+def test_shared_memory_is_handed_back_behind_the_loads_from_it():
+    """A warp that releases a buffer it has loaded from makes the arrival wait for those loads (releaseStage: its address depends on
+    what was loaded); an arrival by itself can overtake them, and the buffer's next contents then come in under the slowest warp."""
+    common = _code("tc_common.cuh")
+    assert "mbarArrive(bar + (used & zero))" in common[common.index("void releaseStage("):]
+    seen = 0
+    for name in SOURCES:
+        code = _code(name)
+        if "mbarInit(&emptyBar[s], VW + 1)" in code or "mbarInit(&empty[i], L::NW)" in code:  # rings that warps with loads release
+            seen += code.count("releaseStage(&empty")
+            assert not re.search(r"mbarArrive\(&empty", code), name
+    assert seen == 4

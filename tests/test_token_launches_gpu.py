@@ -151,3 +151,23 @@ def test_captured_int8_step_accumulates_like_causal_rows(nH, nKV, hd, ctx, growt
     assert ops.device_status() == 0
     # the eight streams' results are put together in another order: a handful of f32 roundings
     assert float((out - want).norm() / want.norm()) < 1e-6
+
+
+@pytest.mark.parametrize("nH,nKV,hd,ctx", [(28, 4, 128, 9000), (9, 1, 128, 4129), (16, 2, 256, 4500), (20, 2, 256, 2049)])
+def test_captured_int8_step_hands_its_buffers_back_behind_their_readers(nH, nKV, hd, ctx):
+    """Several rounds of tiles through the same buffers, a hundred times over: contents that came in under a slow warp's last loads
+    would show as bits that differ from run to run."""
+    s, q, k, v, _ = _int8_session(nH, nKV, hd, ctx, ctx + 300, seed=ctx)
+    pos = torch.tensor([ctx], dtype=torch.int32, device="cuda")
+    qd, kd, vd = dev(q), dev(k[ctx:]), dev(v[ctx:])
+    outs = []
+    for _ in range(2):
+        out = torch.full((1, nH, hd), float("nan"), device="cuda")
+        s.attend(0, qd, kd, vd, out, ctx, dev_pos=pos, graph_capture=True)
+        outs.append(out)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(100):
+        s.attend(0, qd, kd, vd, outs[1], ctx, dev_pos=pos, graph_capture=True)
+        differ += (outs[1] != outs[0]).any()
+    assert differ.item() == 0 and torch.isfinite(outs[0]).all()
+    assert ops.device_status() == 0

@@ -29,6 +29,7 @@ struct DecodeI8Params {
     float invSqrt;
     int directOut;
     unsigned int *err;
+    uint32_t zero;  // 0 (releaseStage)
 };
 
 // One sequence, no partial buffers, the accumulation order of the causal kernel (decode_i8_streams.cu).

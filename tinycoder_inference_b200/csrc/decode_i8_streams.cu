@@ -328,8 +328,10 @@ decodeI8StreamsKernel(const __grid_constant__ DecodeI8Params p) {
                     for (int c = 0; c < 2 * CP; ++c) mmaF16(o[c], x[c][0], x[c][1], x[c][2], x[c][3], b[mt].z, b[mt].w);
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbarArrive(&emptyBar[round & 1u]);
+            uint32_t used = 0u;
+#pragma unroll
+            for (int c = 0; c < 2 * CP; ++c) used ^= __float_as_uint(o[c][0]);
+            releaseStage(&emptyBar[round & 1u], used, p.zero);
         }
     } else {
         // ---------------------------------- row sums ----------------------------------
@@ -357,8 +359,7 @@ decodeI8StreamsKernel(const __grid_constant__ DecodeI8Params p) {
                     ps0 += xv[2 * r], ps1 += xv[2 * r + 1];
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbarArrive(&emptyBar[round & 1u]);
+            releaseStage(&emptyBar[round & 1u], __float_as_uint(l0) ^ __float_as_uint(l1) ^ __float_as_uint(ps0) ^ __float_as_uint(ps1), p.zero);
         }
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) {

@@ -346,15 +346,6 @@ __device__ __forceinline__ float pagedQuery(const PagedAttnParams &p, const PaIt
     return back;
 }
 
-// Hands a stage back once the warp's loads from it have returned.  The arrival alone does not wait for them: with loads still under way it
-// overtook them, and TMA wrote the next tile under the last ldmatrix of the slowest warp (seen as results that differ in a few
-// weights from run to run).  `used` is made of every product that took data of the stage, so that the arrival's address waits for it; zero is
-// a 0 that the compiler does not know.
-__device__ __forceinline__ void releaseStage(uint64_t *bar, uint32_t used, uint32_t zero) {
-    __syncwarp();
-    if ((threadIdx.x & 31u) == 0u) mbarArrive(bar + (used & zero));
-}
-
 // The producer warp of the kernels whose consumers share a tile's rows (paged_rows.cu, paged_steps.cu): hands on the items of the block's run
 // and requests their tiles into the ring, K and V and an int8 store's scales.  L: the kernel's layout.
 template <typename L>

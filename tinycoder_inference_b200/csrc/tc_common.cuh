@@ -122,6 +122,14 @@ __device__ __forceinline__ void mbarExpectTx(uint64_t *bar, uint32_t bytes) {
 __device__ __forceinline__ void mbarArrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smemAddr(bar)) : "memory");
 }
+// Hands a buffer in shared memory back once the warp's loads from it have returned.  The arrival alone does not wait for them: with
+// loads still under way it overtook them, and TMA wrote the next tile under the last ldmatrix of the slowest warp (seen as results of the
+// paged kernels that differ in a few weights from run to run).  `used` is made of every product or sum that took data of the buffer, so
+// that the arrival's address waits for it; zero is a 0 that the compiler does not know.
+__device__ __forceinline__ void releaseStage(uint64_t *bar, uint32_t used, uint32_t zero) {
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0u) mbarArrive(bar + (used & zero));
+}
 // One poll of a phase.  The suspend-time hint lets the hardware park the thread until the phase
 // completes (or the hint runs out) instead of returning at once: a block here has a dozen warps
 // waiting for one another most of the time, and warps that spin through an unhinted try_wait
