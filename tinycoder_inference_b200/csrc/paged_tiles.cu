@@ -34,6 +34,10 @@ constexpr uint32_t kPtOver = 2;
 constexpr int kPtBN = int(kPaTile);
 constexpr float kPtLazyLog2 = 8.0f;  // O is rescaled when the row's maximum ran ahead by 2^8
 constexpr float kPtOff = 6.0f;       // probabilities are held as 2^6 p, at most 2^14: what fp16 has above them goes to the small ones
+// int8: the running maximum counts a tile's V scales as 2^-60 at least.  Scales of 0 would take 2^126 into the probabilities, which f32 does not
+// hold: inf in the row's sum, inf x 0 in P.  At 2^-60 probabilities stay below 2^(60 + 14), what P holds stays below 2^14 as
+// with any larger scale, and what smaller scales add (V below 127 x 2^-60) is 0 in an fp16 result.
+constexpr int kPtLeastScale = -60;
 
 // What a block has of an item, as its producer hands it to the other warps (in shared memory: the walk's state would cost the softmax
 // threads registers that they spill for).  Tiles j = 0 .. nTiles - 1 are cache rows 64 (t0 + j) ..; query tile X takes tile j if
@@ -349,7 +353,8 @@ pagedTilesKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             top = max(top, __float_as_uint(b) & 0x7fffffffu);
                         }
                         top = __reduce_max_sync(0xffffffffu, top);
-                        if (lane == 0) sc[128] = static_cast<float>(static_cast<int>(top >> 23) - 126);  // 2^that is above every scale
+                        // 2^that is above every scale; bounded below, see kPtLeastScale
+                        if (lane == 0) sc[128] = static_cast<float>(max(static_cast<int>(top >> 23) - 126, kPtLeastScale));
                     }
                     if (!pfWait<kCall>(&stFull[s], (gs / (NS ? NS : 1u)) & 1u, err, kDevErrFullWait)) return false;
                     const uint32_t src = smemAddr(smem + L::kStaging + s * L::kKvHalf), dst = smemAddr(smem + (isK ? L::kK : L::kV) + d * L::kKvTile + 2 * h * L::kKvHalf);
