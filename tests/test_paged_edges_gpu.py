@@ -63,3 +63,35 @@ def test_all_v_scales_tiny_or_zero(ws, nH, nKV, hd, scale):
         q = c.normal(c.tokens, nH, hd).half()
         assert (c.attend(q, ws, new) == 0).all()
     assert ops.device_status() == 0
+
+
+def sink(store, nH, nKV, hd, lens, new, drop, seed):
+    """Rows whose weight is 2^-drop of the first row's, which holds V = 0: the small weights are the whole result.  Every q head
+    has a factor of its own near 1, so the weights' roundings differ from head to head and agree within one."""
+    c = Paged(store, nH, nKV, hd, lens, new, 16, seed=seed)
+    q = torch.zeros((c.tokens, nH, hd), device="cuda")
+    q[:, :, 0] = math.sqrt(hd) * math.log(2.0) * (1.0 + torch.arange(nH, device="cuda") / (64.0 * nH))
+    for b, n in enumerate(lens):
+        r = c.rows(b, 0, n)
+        k, v = torch.zeros((n, nKV, hd), device="cuda"), c.normal(n, nKV, hd).abs() + 0.5
+        k[1:, :, 0] = -drop
+        v[0] = 0.0
+        if store == "i8":
+            c.kc.view(-1, nKV, hd)[r] = (k * 4).to(torch.int8)
+            c.ks.view(-1, nKV)[r] = 0.25
+            c.vc.view(-1, nKV, hd)[r] = (v * 20).round().clamp(0, 127).to(torch.int8)
+            c.vs.view(-1, nKV)[r] = 0.04
+        else:
+            c.kc.view(-1, nKV, hd)[r] = k.half()
+            c.vc.view(-1, nKV, hd)[r] = v.half()
+    return c, q
+
+
+@pytest.mark.parametrize("drop", [12, 20, 24])
+@pytest.mark.parametrize("store,nH,nKV,hd", [("f16", 14, 2, 64), ("f16", 28, 4, 128), ("f16", 16, 2, 256), ("i8", 28, 4, 128), ("i8", 16, 2, 256)])
+def test_f32_results_of_small_weights(ws, store, nH, nKV, hd, drop):
+    """A row of large weight that holds nothing, and many of small ones: an f32 result stays one."""
+    for lens, new in (([300], [1]), ([100, 1000], [1, 1]), ([260, 90], [3, 2]), ([700], [40])):
+        c, q = sink(store, nH, nKV, hd, lens, new, drop, seed=drop)
+        c.check(q, c.attend(q, ws, max(new)))
+    assert ops.device_status() == 0

@@ -6,7 +6,8 @@
 // int8 row is turned into fp16 once for all of a block's query rows.  A warp takes 16 of a tile's 64 rows.  What bounds it is the cache for fp16
 // pages and the conversions of int8 ones (two byte permutes, half an exclusive-or and an fp16 subtraction per two values).
 //   * P^T is S^T's accumulator through movmatrix: a thread has keys n8, n8 + 8 of query rows 2 c, 2 c + 1 and needs keys 2 c, 2 c + 1 of row n8.
-//   * The running maximum is lazy: a vote finds whether any score is 2^8 above it, and only then do the lanes exchange maxima and rescale.
+//   * The running maximum is lazy: a vote finds whether any score is 2^8 (f32 results: 2^2) above it, and only then do the lanes exchange
+//     maxima and rescale.
 // Measured (warm graph, tokens of one step): fp16 pages 64 sessions of 40 / 8 / 128 6.5 TB/s, of 40 / 8 / 64 5.8, int8 pages 32 sessions of
 // 512 - 32768 rows of 28 / 4 / 128 5.5 TB/s -- the ALU pipe is half busy with the conversions there, and a warp has a chain of
 // products and exponentials per tile.  One session of 8191 int8 rows takes 15 us, two thirds of it the way from launch to launch.
@@ -18,7 +19,13 @@
 
 namespace tc {
 
-constexpr float kPsOff = 7.0f, kPsLag = 8.0f;  // p is held as 2^7 p, at most 2^15
+// p is held as 2^off p, at most 2^(off + lag) = 2^15: the smallest step of fp16 is 2^-24, so a weight is off by 2^-(25 + off) of the row's
+// largest at most, over int8 pages (p times a scale relative to at most twice the largest) by twice that.  An f32 result may consist of
+// small weights alone, where the large ones meet V = 0: 2^-38 instead of 2^-32 costs more frequent rescales.
+template <bool EXACT>
+struct PsRange {
+    static constexpr float off = EXACT ? 13.0f : 7.0f, lag = EXACT ? 2.0f : 8.0f;
+};
 
 template <int HD, bool I8, bool EXACT, int NT>
 struct PsL {
@@ -227,7 +234,7 @@ pagedStepsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ahead = ahead || s[nt][e] > m[2 * nt + (e & 1)] + kPsLag;
+                for (int e = 0; e < 4; ++e) ahead = ahead || s[nt][e] > m[2 * nt + (e & 1)] + PsRange<EXACT>::lag;
             if (__any_sync(0xffffffffu, ahead)) {
 #pragma unroll
                 for (int r = 0; r < 2 * NT; ++r) {
@@ -247,7 +254,7 @@ pagedStepsKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float mr = m[2 * nt + (e & 1)];
-                    s[nt][e] = fastExp2(s[nt][e] - ((mr == -INFINITY ? 0.0f : mr) - kPsOff));
+                    s[nt][e] = fastExp2(s[nt][e] - ((mr == -INFINITY ? 0.0f : mr) - PsRange<EXACT>::off));
                     l[2 * nt + (e & 1)] += s[nt][e];
                 }
             if constexpr (I8) {
