@@ -95,3 +95,107 @@ def test_f32_results_of_small_weights(ws, store, nH, nKV, hd, drop):
         c, q = sink(store, nH, nKV, hd, lens, new, drop, seed=drop)
         c.check(q, c.attend(q, ws, max(new)))
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 30.0])
+@pytest.mark.parametrize("store,nH,nKV,hd", [("f16", 14, 2, 64), ("f16", 8, 2, 128), ("f16", 16, 2, 256), ("i8", 8, 2, 128), ("i8", 16, 2, 256)])
+def test_flat_and_peaked_rows_of_fp16_queries(ws, store, nH, nKV, hd, scale):
+    """Scores of other sizes, through the forms for few and for many query rows."""
+    for lens, new in (([700, 90], [1, 1]), ([700, 90], [2, 9]), ([2500, 128], [20, 40]), ([1900, 300], [150, 300])):
+        c = Paged(store, nH, nKV, hd, lens, new, 16, seed=3)
+        q = c.normal(c.tokens, nH, hd).half()
+        for most in (max(new), 0):
+            c.check(q, c.attend(q, ws, most, scale=scale / math.sqrt(hd)), scale / math.sqrt(hd))
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("store,hd", [("f16", 64), ("f16", 128), ("f16", 256), ("i8", 128), ("i8", 256)])
+@pytest.mark.parametrize("io", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rising", [True, False])
+def test_scores_that_rise_or_fall_along_a_sequence(ws, store, hd, io, rising):
+    """Every tile moves the running maximum, or none behind the first one does."""
+    for lens, new in (([2000], [1]), ([1500, 400], [4, 4]), ([1300, 500], [130, 30])):
+        c = Paged(store, 8, 2, hd, lens, new, 16, seed=7)
+        q = c.normal(c.tokens, 8, hd).to(io)
+        q[:, :, 0] = 0.5 * math.sqrt(hd)
+        for b, n in enumerate(lens):
+            r = c.rows(b, 0, n)
+            ramp = torch.linspace(-30.0, 30.0, n, device="cuda") * (1.0 if rising else -1.0)
+            if store == "i8":
+                c.ks.view(-1, 2)[r] = 0.25
+                c.kc.view(-1, 2, hd)[r] = (c.normal(n, 2, hd) * 4).round().clamp(-8, 8).to(torch.int8)
+                c.kc.view(-1, 2, hd)[r, :, 0] = (ramp * 4).round().to(torch.int8)[:, None]
+            else:
+                c.kc.view(-1, 2, hd)[r, :, 0] = ramp.half()[:, None]
+        c.check(q, c.attend(q, ws, max(new)))
+    assert ops.device_status() == 0
+
+
+class Without(Paged):
+    """A cache whose first sequence has a table entry outside the pool and whose second one has a length past its table."""
+
+    def spoil(self, page):
+        self.pages[0, self.lens_h[0] // self.page // 2] = page
+        self.lens[1] = self.pages.shape[1] * self.page + 5
+
+
+@pytest.mark.parametrize("store,hd", [("f16", 64), ("f16", 128), ("f16", 256), ("i8", 128), ("i8", 256)])
+@pytest.mark.parametrize("io", [torch.float16, torch.float32])
+@pytest.mark.parametrize("new", [1, 3, 40, 200])
+def test_bad_tables_touch_nothing_else(ws, store, hd, io, new):
+    """Entries that name no page and lengths past the table are reported; other sequences' results and tokens of no sequence are as they
+    were, whichever form takes the call, K and V and the scales of an int8 row."""
+    for page in (1 << 30, -1, -2 ** 31):
+        c = Without(store, 8, 2, hd, [900, 700, 800, 450], [new] * 4, 16, seed=new)
+        q = torch.zeros((c.tokens + 5, 8, hd), device="cuda", dtype=io)
+        q[:c.tokens] = c.normal(c.tokens, 8, hd).to(io)
+        out = torch.full_like(q, 5.0)
+        c.spoil(page)
+        ops.attn_paged(q, c.kc, c.vc, c.pages, c.lens, out, ws, starts=c.starts, max_tokens=new, ks=c.ks, vs=c.vs)
+        assert ops.device_status(raise_on_flags=False) == 32
+        assert (out[c.tokens:] == 5.0).all()
+        c.lens_h, c.new_h, c.pages = c.lens_h[2:], c.new_h[2:], c.pages[2:]
+        c.check(q[2 * new:4 * new], out[2 * new:4 * new])
+        assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("store", ["f16", "i8"])
+def test_bad_tables_of_the_writer_and_the_reader(store):
+    """Rows without a page are not stored and read back as zeros; all others are what they are without them."""
+    nKV, hd, new = 2, 128, 100
+    c = Without(store, 8, nKV, hd, [300, 300, 300], [new] * 3, 16, seed=1, fill=False)
+    k, v = c.normal(c.tokens, nKV, hd), c.normal(c.tokens, nKV, hd)
+    c.pages[0, 300 // 16 - 1] = -1           # rows 272 .. 287 of the first sequence
+    c.lens[1] = c.pages.shape[1] * 16 + 5    # the second one's last five rows lie past the table
+    pools = [t.clone() if t is not None else None for t in (c.kc, c.vc, c.ks, c.vs)]
+    ops.paged_write(k, v, c.kc, c.vc, c.pages, c.lens, starts=c.starts, ks=c.ks, vs=c.vs)
+    assert ops.device_status(raise_on_flags=False) == 32
+    ko, vo = torch.full_like(k, 9.0), torch.full_like(v, 9.0)
+    ops.paged_read(c.kc, c.vc, c.pages, c.lens, ko, vo, starts=c.starts, ks=c.ks, vs=c.vs)
+    assert ops.device_status(raise_on_flags=False) == 32
+    lost = torch.zeros(c.tokens, dtype=torch.bool, device="cuda")
+    lost[72:88] = True                       # tokens at rows 272 .. 287 (tokens 0 .. 99 are rows 200 .. 299)
+    lost[195:200] = True
+    for got, x, pool, old in ((ko, k, c.kc, pools[0]), (vo, v, c.vc, pools[1])):
+        assert (got[lost] == 0).all()
+        if store == "f16":
+            assert torch.equal(got[~lost], x[~lost].half().float())
+        else:  # half a step of a row's largest / 127
+            assert ((got - x)[~lost].abs() <= x[~lost].abs().amax(-1, keepdim=True) / 127 * 0.5001).all()
+        # stored rows: those that were not lost, no others
+        changed = (pool.view(-1, nKV * hd) != old.view(-1, nKV * hd)).any(-1) & ~(torch.isnan(pool.view(-1, nKV * hd).float()).all(-1))
+        assert changed.sum().item() == (~lost).sum().item()
+
+
+@pytest.mark.parametrize("store,io", [("f16", torch.float32), ("f16", torch.float16), ("i8", torch.float32), ("i8", torch.float16)])
+def test_values_of_tokens_between_tokens_of_no_sequence(ws, store, io):
+    """`starts` that begin behind the first token and end ahead of the last one, with the items of a long prompt."""
+    tokens, hd = 4000, 128
+    c = Paged(store, 8, 4, hd, [tokens, 40], [tokens - 9, 3], 16, seed=6)
+    c.starts += 4
+    q = c.normal(tokens, 8, hd).to(io)
+    out = torch.full_like(q, 5.0)
+    ops.attn_paged(q, c.kc, c.vc, c.pages, c.lens, out, ws, starts=c.starts, ks=c.ks, vs=c.vs)
+    assert (out[:4] == 5).all() and (out[tokens - 2:] == 5).all()
+    c.check(q[4:tokens - 2], out[4:tokens - 2])
+    assert ops.device_status() == 0
