@@ -199,3 +199,70 @@ def test_values_of_tokens_between_tokens_of_no_sequence(ws, store, io):
     assert (out[:4] == 5).all() and (out[tokens - 2:] == 5).all()
     c.check(q[4:tokens - 2], out[4:tokens - 2])
     assert ops.device_status() == 0
+
+
+def off(x):
+    """The same values at an address that is a multiple of 16 bytes and not of 32."""
+    n = 16 // x.element_size()
+    flat = torch.empty(x.numel() + 3 * n, dtype=x.dtype, device="cuda")
+    at = n if flat.data_ptr() % 32 == 0 else 2 * n
+    y = flat[at:at + x.numel()].view(x.shape)
+    y.copy_(x)
+    assert y.data_ptr() % 32 == 16
+    return y
+
+
+@pytest.mark.parametrize("store,hd", [("f16", 64), ("f16", 128), ("f16", 256), ("i8", 128), ("i8", 256)])
+@pytest.mark.parametrize("io", [torch.float16, torch.float32])
+def test_arrays_at_16_bytes(ws, store, hd, io):
+    """Every array at an odd multiple of 16 bytes, through every form: the same bits as at wider alignments."""
+    other = off(ws)
+    for lens, new in (([300, 65], [1, 1]), ([900, 65], [3, 2]), ([1200, 65], [40, 60]), ([1500, 400], [200, 400])):
+        c = Paged(store, 8, 2, hd, lens, new, 16, seed=new[0])
+        q = c.normal(c.tokens, 8, hd).to(io)
+        k, v, cos = c.normal(c.tokens, 2, hd), c.normal(c.tokens, 2, hd), c.normal(max(lens), hd // 2)
+        results = []
+        for place in (lambda t: t, off):
+            kc, vc, qq, out, q32, q_out = (place(t) for t in (c.kc.clone(), c.vc.clone(), q, torch.zeros_like(q), q.float(), torch.zeros_like(q)))
+            ks, vs = (t.clone() if t is not None else None for t in (c.ks, c.vs))
+            w = ws if place is not off else other
+            ops.attn_paged(qq, kc, vc, c.pages, c.lens, out, w, starts=c.starts, max_tokens=max(new), ks=ks, vs=vs)
+            ops.paged_write(place(k), place(v), kc, vc, c.pages, c.lens, starts=c.starts, ks=ks, vs=vs, q=q32, q_out=q_out, cosT=place(cos), sinT=place(cos))
+            ko, vo = place(torch.zeros_like(k).to(io)), place(torch.zeros_like(k).to(io))
+            ops.paged_read(kc, vc, c.pages, c.lens, ko, vo, starts=c.starts, ks=ks, vs=vs)
+            results.append([out, q_out, ko, vo])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        c.check(q, results[1][0])
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("io", [torch.float16, torch.float32])
+@pytest.mark.parametrize("store", ["f16", "i8"])
+def test_a_page_of_two_sequences(ws, store, io):
+    """Sequences that share the pages of a common beginning (and one that has a page twice): each as if they were its own."""
+    for new in (1, 3, 40, 150):
+        c = Paged(store, 8, 2, 128, [700, 700, 700], [new] * 3, 32, seed=new)
+        c.pages[1, :15] = c.pages[0, :15]
+        c.pages[2, 3] = c.pages[2, 9]
+        q = c.normal(c.tokens, 8, 128).to(io)
+        c.check(q, c.attend(q, ws, new))
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("store,io", [("f16", torch.float16), ("i8", torch.float16), ("i8", torch.float32)])
+def test_calls_of_one_workspace_behind_each_other(store, io):
+    """Calls of different forms and sizes in a row, nothing between them: each takes the workspace as the one before left it."""
+    w = ops.paged_workspace()
+    calls = []
+    for seed, (lens, new) in enumerate((([3000, 90], [1, 1]), ([2500], [300]), ([40, 3000, 7], [3, 2, 7]), ([1], [1]), ([2000] * 40, [1] * 40), ([1500, 900], [700, 1]))):
+        c = Paged(store, 28, 4, 128, lens, new, 16, seed=seed)
+        q = c.normal(c.tokens, 28, 128).to(io)
+        calls.append((c, q, torch.full_like(q, 9.0)))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for c, q, out in calls:
+            ops.attn_paged(q, c.kc, c.vc, c.pages, c.lens, out, w, starts=c.starts, max_tokens=max(c.new_h), ks=c.ks, vs=c.vs)
+    for c, q, out in calls:
+        c.check(q, out)
+    assert ops.device_status() == 0
