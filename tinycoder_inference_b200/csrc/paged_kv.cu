@@ -152,7 +152,7 @@ struct PagedReadParams {
     const void *kc, *vc;
     const float *ks, *vs;
     void *kOut, *vOut;
-    uint32_t unitsPerToken, out32;  // out32: the outputs are 32-byte aligned
+    uint32_t out32;  // the outputs are 32-byte aligned
 };
 
 // 16 bytes of a store row as f32 or fp16 values from element `at` on
@@ -193,10 +193,10 @@ __device__ __forceinline__ void pagedPut(void *out, size_t at, const uint4 &raw,
 // starts -> lens -> page -> row is all there is.
 template <int HD, bool I8, bool HALF>
 __global__ void __launch_bounds__(256) pagedReadKernel(const __grid_constant__ PagedReadParams p) {
-    constexpr uint32_t E = I8 ? 16 : 8, G = HD / E, U = 1;  // values of a lane; lanes of a row; rows of a group
+    constexpr uint32_t E = I8 ? 16 : 8, G = HD / E;  // values of a lane; lanes of a row
     const uint32_t unit = blockIdx.x * (256u / G) + threadIdx.x / G;
     const uint32_t i = threadIdx.x & (G - 1u);
-    const uint32_t t = unit / p.unitsPerToken, first = (unit - t * p.unitsPerToken) * U;
+    const uint32_t rows = 2u * p.c.nKV, t = unit / rows, r = unit - t * rows;  // row r of token t: K heads, then V heads
     gridDepWait();
     gridDepLaunch();
     if (t >= p.c.tokens) return;
@@ -204,30 +204,17 @@ __global__ void __launch_bounds__(256) pagedReadKernel(const __grid_constant__ P
     int64_t pos;
     if (!findToken<G>(p.c, t, seq, pos)) return;
     size_t row = 0;
-    const bool held = pagedRow(p.c, seq, pos, row);
+    const bool held = pagedRow(p.c, seq, pos, row), isV = r >= p.c.nKV;
     if (!held && i == 0) atomicOr(p.c.err, kDevErrRowBound);
-    uint4 raw[U];
-    float sc[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t r = first + u;
-        raw[u] = make_uint4(0u, 0u, 0u, 0u);  // a row without a page reads as zero
-        sc[u] = 0.0f;
-        if (r >= 2u * p.c.nKV || !held) continue;
-        const bool isV = r >= p.c.nKV;
-        const size_t rowHead = row * p.c.nKV + (isV ? r - p.c.nKV : r);
-        raw[u] = __ldg(static_cast<const uint4 *>(isV ? p.vc : p.kc) + rowHead * G + i);
-        if (I8) sc[u] = __ldg((isV ? p.vs : p.ks) + rowHead);
+    const uint32_t head = isV ? r - p.c.nKV : r;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);  // a row without a page reads as zero
+    float sc = 0.0f;
+    if (held) {
+        const size_t rowHead = row * p.c.nKV + head;
+        raw = __ldg(static_cast<const uint4 *>(isV ? p.vc : p.kc) + rowHead * G + i);
+        if (I8) sc = __ldg((isV ? p.vs : p.ks) + rowHead);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t r = first + u;
-        if (r >= 2u * p.c.nKV) continue;
-        const bool isV = r >= p.c.nKV;
-        const size_t at = ((static_cast<size_t>(t) * p.c.nKV + (isV ? r - p.c.nKV : r)) * G + i) * E;
-        void *out = isV ? p.vOut : p.kOut;
-        pagedPut<I8, HALF>(out, at, raw[u], sc[u], p.out32 != 0u);
-    }
+    pagedPut<I8, HALF>(isV ? p.vOut : p.kOut, ((static_cast<size_t>(t) * p.c.nKV + head) * G + i) * E, raw, sc, p.out32 != 0u);
 }
 
 // The same for many rows: a block takes kReadTokens tokens.  One warp looks them up, a lane each, and leaves their rows in shared memory; then
@@ -353,15 +340,13 @@ int tc_paged_kv_read(const tc_paged_kv *c, void *kOut, void *vOut, int outHalf, 
     TC_REQUIRE(((reinterpret_cast<uintptr_t>(kOut) | reinterpret_cast<uintptr_t>(vOut)) & 15u) == 0, TC_EINVAL, "paged read: alignment (16 bytes)");
     unsigned int *err = devErrorWord();
     TC_REQUIRE(err != nullptr, TC_ECUDA, "no CUDA device");
-    PagedReadParams p{pagedView(c, err), c->k, c->v, c->ks, c->vs, kOut, vOut, 0, 0};
+    PagedReadParams p{pagedView(c, err), c->k, c->v, c->ks, c->vs, kOut, vOut, 0};
     p.out32 = ((reinterpret_cast<uintptr_t>(kOut) | reinterpret_cast<uintptr_t>(vOut)) & 31u) == 0;
     const uint32_t rows = 2 * c->nKV, lanes = c->hd / (c->kvI8 ? 16 : 8);
     const bool many = manyRows(static_cast<uint64_t>(c->tokens) * rows, lanes);
-    p.unitsPerToken = rows;
-    uint32_t blocks;
-    const int gc = pagedGrid(static_cast<uint64_t>(c->tokens) * rows, lanes, &blocks);
+    uint32_t blocks = (c->tokens + kReadTokens - 1) / kReadTokens;
+    const int gc = many ? TC_OK : pagedGrid(static_cast<uint64_t>(c->tokens) * rows, lanes, &blocks);
     if (gc != TC_OK) return gc;
-    if (many) blocks = (c->tokens + kReadTokens - 1) / kReadTokens;
     auto go = [&](auto kern) { return launchDependent(kern, dim3(blocks), 256, 0, static_cast<cudaStream_t>(stream), 1, p); };
 #define TC_PAGED_READ(HD, I8) \
     (many ? (outHalf ? go(pagedReadManyKernel<HD, I8, true>) : go(pagedReadManyKernel<HD, I8, false>)) \
