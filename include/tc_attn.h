@@ -465,12 +465,20 @@ int tc_paged_kv_read(const tc_paged_kv *c, void *kOut, void *vOut, int outHalf,
 
 /* Causal attention of the new tokens over their sequences' rows (already written): the
  * token at row r sees rows [0, r]; one that sees none gives zeros.  q / out
- * [tokens][nHeads][hd], both f32 (results to f32 accuracy whatever the store) or both
- * fp16 (half != 0: fp16 products, f32 sums and softmax).  maxTokens: the most
- * new tokens of a sequence as far as the caller knows (0: unknown); it chooses the
- * form of the launch, not the result's meaning.  Steps of one token, drafts, chunks and whole
- * prompts may share a call.  Rows [0, lens[b]) have to hold finite numbers; what
- * lies behind them may be anything.
+ * [tokens][nHeads][hd], both f32 or both fp16 (half != 0).  Steps of one token, drafts, chunks
+ * and whole prompts may share a call.  Rows [0, lens[b]) have to hold finite numbers, scales of at
+ * most 2^100 (0 is one); what lies behind them may be anything.
+ *   f32: results to f32 accuracy whatever the store.  A weight is held to 2^-21 of itself or to
+ * 2^-38 of its row's largest, over int8 pages to 2^-37 of the largest one times the sequence's largest V
+ * scale, whichever is more.
+ *   fp16: fp16 products, f32 softmax and sums.  A weight is rounded to 2^-11 of itself or to 2^-31 of its
+ * row's largest (int8: 2^-30, with the scales as above).  Over V the tensor unit sums 16 rows at a time and cuts off
+ * what an addition shifts out: up to 2^-23 of the sum per 16 rows that one block sums up, half of that as a
+ * rule (one step of fp16 behind 113000 rows).
+ * maxTokens: the most new tokens of a sequence as far as the caller knows; it chooses the form of
+ * the launch, not the result's meaning.  0 (unknown): with starts the call is launched as if one
+ * sequence might bring all its tokens, and a step of 32 - 64 sessions takes 15 - 60 percent longer than
+ * with 1.
  * workspace: tc_attn_paged_workspace_bytes, 16-byte aligned, whatever it holds; calls that
  * may overlap need one each.
  * At most 128 q heads per kv head. */

@@ -45,7 +45,9 @@ struct PagedAttnParams {
 __device__ __forceinline__ uint64_t divide(uint64_t a, uint64_t b) {
     return ((a | b) >> 32) == 0u ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
-// sum of (a i + b) / m over i = 0 .. n - 1, rounded down each: term by term while there are few, else by Euclid's steps on (a, m)
+// sum of (a i + b) / m over i = 0 .. n - 1, rounded down each: term by term while there are few, else by Euclid's steps on (a, m):
+// the lattice points under a line, counted by exchanging the axes (the reciprocity of floor sums in Graham, Knuth and Patashnik,
+// Concrete Mathematics, 3.5)
 __device__ __forceinline__ uint64_t floorSum(uint32_t n, uint32_t m, uint32_t a, uint64_t b0) {
     uint64_t sum = 0;
     if (n <= 24u) {

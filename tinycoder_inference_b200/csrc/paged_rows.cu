@@ -16,7 +16,8 @@
 
 namespace tc {
 
-constexpr float kPrOff = 13.0f;  // p is held as 2^13 p: its fp16 pair keeps 11 + 11 bits down to p = 2^-27
+// p is held as 2^13 p: its fp16 pair keeps 11 + 11 bits down to p = 2^-15, the upper half's 11 down to 2^-27, and is off by 2^-38 at most
+constexpr float kPrOff = 13.0f;
 
 template <int HD>
 struct PrL {

@@ -63,11 +63,14 @@ int getTensorMap(const TensorMapKey &key, CUtensorMap *out);
 
 // Launch under programmatic dependent launch: the grid may be scheduled while the one in front of it drains, so
 // the kernel has to call gridDepWait() before it touches anything that grid may have written or may still read --
-// every kernel launched through here does so first thing (hints towards L2 may go ahead of it), but for the int8 decode at head_dim 128 under
-// TC_DECODE_PDL, which requests rows of its pool that the caller calls old (prefetchRows) ahead of it.  Where the others
-// call gridDepLaunch() decides what such a launch may find unfinished:
+// every kernel launched through here does so first thing (hints towards L2 may go ahead of it), but for
+//   * the int8 decode at head_dim 128 under TC_DECODE_PDL, which requests rows of its pool that the caller calls old (prefetchRows) ahead of it;
+//   * the three kernels of paged attention, whose producers take a first look at lens and starts ahead of it (PagedWalk::prepare).  They
+//     read them through L2, make nothing of them but what the block's run is, and look again behind the wait (PagedWalk::start):
+//     what has changed is worked out anew.
+// Where the others call gridDepLaunch() decides what such a launch may find unfinished:
 //   * after the wait, so that the kernels ahead of theirs are complete;
-//   * a kernel that writes int8 rows of head_dim 128 (nothing else is read ahead of a wait), not before those are in
+//   * a kernel that writes int8 rows of head_dim 128 (nothing else is taken ahead of a wait for good), not before those are in
 //     memory: kvQuantKernel by its exit, a decode kernel that takes the new row along behind that row's store.  The rows
 //     launch of a prompt may let the next grid in sooner: that is the attention launch, which waits before it does.
 // So a row written by any call without TC_DECODE_PDL is in memory before a call behind it can look.  (In stream order a dependent launch takes 3.1 - 3.7 us on

@@ -293,7 +293,8 @@ def paged_workspace(device=None):
 
 def attn_paged(q, kc, vc, pages, lens, out, ws, starts=None, max_tokens=0, ks=None, vs=None, invSqrt=None):
     """Causal attention of the new tokens over their sequences' rows.  q, out [tokens][nHeads][hd], both f32 or both
-    fp16.  max_tokens: the most new tokens of a sequence as far as the caller knows (0: unknown)."""
+    fp16.  max_tokens: the most new tokens of a sequence as far as the caller knows; 0: unknown, which with starts costs
+    a step of one token for each of many sequences 15 - 60 percent."""
     check(_n.attn_paged(kc, vc, ks, vs, pages, lens, starts, q, out, ws, max_tokens, invSqrt))
 
 
