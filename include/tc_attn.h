@@ -473,8 +473,8 @@ int tc_paged_kv_read(const tc_paged_kv *c, void *kOut, void *vOut, int outHalf,
  * scale, whichever is more.
  *   fp16: fp16 products, f32 softmax and sums.  A weight is rounded to 2^-11 of itself or to 2^-31 of its
  * row's largest (int8: 2^-30, with the scales as above).  Over V the tensor unit sums 16 rows at a time and cuts off
- * what an addition shifts out: up to 2^-23 of the sum per 16 rows that one block sums up, half of that as a
- * rule (one step of fp16 behind 113000 rows).
+ * what an addition shifts out: up to 2^-23 of the sum per 16 rows that one block sums up, some 2^-25 as a
+ * rule (half a step of fp16 behind 113000 rows).
  * maxTokens: the most new tokens of a sequence as far as the caller knows; it chooses the form of
  * the launch, not the result's meaning.  0 (unknown): with starts the call is launched as if one
  * sequence might bring all its tokens, and a step of 32 - 64 sessions takes 15 - 60 percent longer than

@@ -4,15 +4,17 @@
 // The work, the ring and the partials are paged_attn.cuh's; the products have the cache rows on the M side of mma.sync m16n8k16: S^T = K Q^T
 // (16 cache rows x 8 query rows) and O^T += V^T P^T (16 dims x 8 query rows), so that 8 query rows fill an instruction and an
 // int8 row is turned into fp16 once for all of a block's query rows.  A warp takes 16 of a tile's 64 rows.  What bounds it is the cache for fp16
-// pages and the conversions of int8 ones (two byte permutes, half an exclusive-or and an fp16 subtraction per two values).
+// pages; over int8 ones no unit by itself but a warp's chain per tile, the conversions in it (two byte permutes, half an exclusive-or and an
+// fp16 subtraction per two values).
 //   * P^T is S^T's accumulator through movmatrix: a thread has keys n8, n8 + 8 of query rows 2 c, 2 c + 1 and needs keys 2 c, 2 c + 1 of row n8.
 //   * The running maximum is lazy: a vote finds whether any score is 2^8 (f32 results: 2^2) above it, and only then do the lanes exchange
 //     maxima and rescale.
 // Measured (warm graph, tokens of one step): fp16 pages 64 sessions of 40 / 8 / 128 6.5 TB/s, of 40 / 8 / 64 5.8, int8 pages 32 sessions of
-// 512 - 32768 rows of 28 / 4 / 128 5.5 TB/s -- the ALU pipe is half busy with the conversions there, and a warp has a chain of
-// products and exponentials per tile.  One session of 8191 int8 rows takes 15 us, two thirds of it the way from launch to launch.
+// 512 - 32768 rows of 28 / 4 / 128 5.5 TB/s, with the ALU pipe and the issue slots half busy.  One session of 8191 int8 rows
+// takes 15.5 us, two thirds of it the way from launch to launch.
 //   * EXACT (f32 results): q and p as fp16 pairs, hi and lo in two products; the products of a tile are summed by themselves and join f32 registers,
-//     since the tensor unit cuts off what an addition shifts out.  fp16 results accumulate in the instruction.
+//     since the tensor unit cuts off what an addition shifts out.  fp16 results accumulate in the instruction: some 2^-25 of
+//     the sum lost per tile (a warp's 16 rows), 2^-14 behind 113000 rows of one block.
 #include <algorithm>
 
 #include "paged_attn.cuh"
